@@ -17,7 +17,7 @@
 
 enum TkCheckedKernel : int {
     TK_K_GATHER = 1, TK_K_QK_ROPE = 2, TK_K_ATTN_GENERIC = 3, TK_K_ATTN_TILES = 4, TK_K_CONV = 5,
-    TK_K_SKINNY_CONV = 6,
+    TK_K_SKINNY_CONV = 6, TK_K_KV8_WRITE = 7, TK_K_KV8_ATTN = 8,
 };
 enum TkCheckedIndex : int { TK_CHK_PAGE = 1, TK_CHK_SLOT = 2, TK_CHK_ROW = 3 };
 

@@ -23,6 +23,7 @@ __all__ = [
     "attention_prefill_tc_status",
     "conv_gated", "conv_min_tile",
     "gemm", "gemm_skinny", "gemm_skinny_conv", "gemm_skinny_ok", "gemm_tc", "gemm_tc_ok", "gemm_tc_status", "sample", "sample_status", "gather_rows_select",
+    "qk_norm_rope_write8", "kv8_supported", "attention_kv8_decode", "attention_kv8_prefill", "attention_kv8_tokens", "copy_rows",
 ]
 
 
@@ -51,7 +52,8 @@ def set_check_bounds(pages: int, slots: int) -> None:
 
 
 CHECKED_KERNELS = {1: "row gather", 2: "q/k norm + rope + cache write", 3: "attention (generic)",
-                   4: "attention (tensor cores)", 5: "gated short conv", 6: "projection with the conv inside"}
+                   4: "attention (tensor cores)", 5: "gated short conv", 6: "projection with the conv inside",
+                   7: "8-bit cache write", 8: "attention (8-bit cache)"}
 CHECKED_INDICES = {1: "page", 2: "state row", 3: "table row"}
 
 
@@ -1958,3 +1960,8 @@ def attention_biased_mma(q: torch.Tensor, kv_pool: torch.Tensor, out: torch.Tens
               n_tiles, _ptr(_i32(singles, "singles")) if singles is not None else None, int(n_single), int(nsplit), _ptr(part_o),
               _ptr(part_ml), H, Hkv, D, Dv, Dp, P, int(window or 0), float(scale), float(cap or 0.0), *_bias_table(bias_log2, H),
               int(bool(bounded)), int(bool(sink)), _stream())
+
+
+# the 8-bit cache's operators (they use the helpers above)
+from tokenomos_b200.ops.kv8 import (attention_kv8_decode, attention_kv8_prefill, attention_kv8_tokens, copy_rows,  # noqa: E402
+                                    kv8_supported, qk_norm_rope_write8)

@@ -1,0 +1,185 @@
+"""The 8-bit cache's operators: the quantised write, attention over it, and the copying of cache rows.
+
+A paged state of such a cache is two tensors: ``pool`` [pages, 2, kv_heads, page, head_dim] of ``torch.float8_e4m3fn`` and
+``scales`` [pages, 2, kv_heads] float32, one power of two for each block (the positions of a page, keys or values, one KV
+head). A byte stands for ``scale * e4m3``; a block's scale is the smallest with which its largest magnitude fits (between
+2^-40 and 2^40). A token whose keys or values of a head are not finite, or above 448 * 2^40, is marked: what sees it is NaN.
+"""
+
+from __future__ import annotations
+
+import array
+import ctypes
+from typing import Sequence
+
+import torch
+
+from tokenomos_b200 import ops
+from tokenomos_b200.ops import _lib
+from tokenomos_b200.ops._lib import KernelError
+
+KV8_DTYPE = torch.float8_e4m3fn
+
+
+def _here(name: str, *tensors: torch.Tensor | None) -> None:
+    """Every tensor on the current device, whose stream the launch goes to."""
+    ops._cuda(*tensors)
+    now = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != now:
+            raise KernelError(f"{name}: a tensor on {t.device} while cuda:{now} is the current device")
+
+
+def _check_cache(name: str, pool: torch.Tensor, scales: torch.Tensor) -> tuple[int, int, int]:
+    """(kv_heads, page, head_dim) of an 8-bit cache."""
+    if pool.dtype != KV8_DTYPE or pool.dim() != 5 or pool.shape[1] != 2 or not pool.is_contiguous():
+        raise KernelError(f"{name}: the cache is a contiguous {KV8_DTYPE} [pages, 2, kv_heads, page, head_dim] tensor, "
+                          f"got {pool.dtype} {tuple(pool.shape)}")
+    if scales.dtype != torch.float32 or scales.shape != pool.shape[:3] or not scales.is_contiguous():
+        raise KernelError(f"{name}: the scales are a contiguous float32 {tuple(pool.shape[:3])} tensor, got "
+                          f"{scales.dtype} {tuple(scales.shape)}")
+    return pool.shape[2], pool.shape[3], pool.shape[4]
+
+
+def _check_layout(name: str, tokens: int, positions: torch.Tensor, tok_seq: torch.Tensor, block_table: torch.Tensor) -> None:
+    for what, t in (("positions", positions), ("tok_seq", tok_seq)):
+        if ops._i32(t, what).numel() < tokens:
+            raise KernelError(f"{name}: {what} is shorter than the {tokens} rows")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise KernelError(f"{name}: block_table is an int32 [sequences, blocks] tensor with contiguous rows")
+
+
+def kv8_supported(heads: int, kv_heads: int, head_dim: int) -> bool:
+    """Whether the 8-bit cache's operators take a layer: heads of 64 or 128, at most 16 query heads a KV head."""
+    return bool(_lib.call("tk_attn_kv8_supported", heads, kv_heads, head_dim))
+
+
+def qk_norm_rope_write8(qkv: torch.Tensor, pool: torch.Tensor, scales: torch.Tensor, wq: torch.Tensor | None,
+                        wk: torch.Tensor | None, eps: float, inv_freq: torch.Tensor, positions: torch.Tensor,
+                        tok_seq: torch.Tensor, block_table: torch.Tensor, heads: int, kv_heads: int, head_dim: int, page: int,
+                        cs_mult: float = 1.0, interleaved: bool = False) -> torch.Tensor:
+    """``qk_norm_rope_write`` for an 8-bit cache: norm (``wq``, ``wk``: both or neither) and rotate the q and k heads of
+    ``qkv`` [T, (H + 2 Hkv) D] (rows may be strided); returns q [T, H, D] and writes k and v into ``pool`` and ``scales`` at each token's
+    position. ``inv_freq`` [R / 2]: the first R columns are rotated, pairs (i, i + R / 2), or (2i, 2i + 1) when
+    ``interleaved``; cos and sin are multiplied by ``cs_mult``. Everything is 32-bit (angles 64-bit) and rounded once.
+
+    A sequence's tokens lie side by side in the step, at consecutive positions, and a page that tokens are written into
+    belongs to one sequence. A block that already holds tokens of earlier steps keeps its scale or raises it, and then its earlier bytes are
+    rounded to the new one (which changes nothing above 2^-6 of it, e4m3's smallest normal number)."""
+    name = "qk_norm_rope_write8"
+    _here(name, qkv, pool, scales, wq, wk, inv_freq, positions, tok_seq, block_table)
+    if _check_cache(name, pool, scales) != (kv_heads, page, head_dim):
+        raise KernelError(f"{name}: cache {tuple(pool.shape)} does not match [pages, 2, {kv_heads}, {page}, {head_dim}]")
+    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] != (heads + 2 * kv_heads) * head_dim:
+        raise KernelError(f"{name}: qkv {tuple(qkv.shape)} for {heads}+2*{kv_heads} heads of {head_dim}")
+    code = ops._dtype_code(qkv)
+    T = qkv.shape[0]
+    _check_layout(name, T, positions, tok_seq, block_table)
+    rot = 2 * inv_freq.numel()
+    ops._f32vec(inv_freq, "inv_freq", rot // 2)
+    q = torch.empty(T, heads, head_dim, dtype=qkv.dtype, device=qkv.device)
+    _lib.call("tk_qk_norm_rope_write8", qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1], q.data_ptr(), pool.data_ptr(),
+              scales.data_ptr(), ops._ptr(ops._f32vec(wq, "q_norm weight", head_dim)), ops._ptr(ops._f32vec(wk, "k_norm weight", head_dim)),
+              float(eps), inv_freq.data_ptr(), float(cs_mult), int(bool(interleaved)), positions.data_ptr(), tok_seq.data_ptr(),
+              block_table.data_ptr(), block_table.stride(0), T, heads, kv_heads, head_dim, rot, page, code, ops._stream())
+    return q
+
+
+def _check_attention(name, q, pool, scales, out, positions, tok_seq, block_table, gate):
+    _here(name, q, pool, scales, out, positions, tok_seq, block_table, gate)
+    Hkv, P, D = _check_cache(name, pool, scales)
+    if (q.dim() != 3 or q.shape[2] != D or q.shape[1] % Hkv or out.shape != q.shape or out.dtype != q.dtype
+            or not (q.is_contiguous() and out.is_contiguous())):
+        raise KernelError(f"{name}: contiguous q and out [T, H, {D}] of one type, H a multiple of {Hkv}; got {tuple(q.shape)} "
+                          f"{q.dtype} and {tuple(out.shape)} {out.dtype}")
+    T, H, _ = q.shape
+    code = ops._dtype_code(q)
+    _check_layout(name, T, positions, tok_seq, block_table)
+    if gate is not None and (gate.dtype != q.dtype or tuple(gate.shape) != (T, H) or gate.stride(1) != 1):
+        raise KernelError(f"{name}: gate must be a {q.dtype} [T, {H}] view with unit column stride")
+    return T, H, Hkv, P, D, code
+
+
+_sm_count: dict = {}
+
+
+def _sms(device: torch.device) -> int:
+    n = _sm_count.get(device)
+    if n is None:
+        n = _sm_count[device] = torch.cuda.get_device_properties(device).multi_processor_count
+    return n
+
+
+def _attend(q, pool, scales, out, positions, tok_seq, block_table, tok0, ntok, items, rows, shape, window, scale, longest, gate, sink):
+    T, H, Hkv, P, D, code = shape
+    reach = abs(int(window)) if window else longest
+    nsplit = _lib.call("tk_attn_kv8_splits", items, Hkv, max(1, min(int(longest), reach + rows)), _sms(q.device))
+    scratch = None
+    if nsplit > 1:
+        scratch = torch.empty(items * Hkv * nsplit * rows * (H // Hkv) * (D + 4), dtype=torch.float32, device=q.device)
+    _lib.call("tk_attn_kv8", q.data_ptr(), pool.data_ptr(), scales.data_ptr(), out.data_ptr(), positions.data_ptr(), tok_seq.data_ptr(),
+              block_table.data_ptr(), block_table.stride(0), ops._ptr(tok0), ops._ptr(ntok), items, H, Hkv, D, P, int(window or 0),
+              float(scale), nsplit, ops._ptr(scratch), ops._ptr(gate), gate.stride(0) if gate is not None else 0, int(bool(sink)), code,
+              ops._stream())
+
+
+def attention_kv8_decode(q: torch.Tensor, pool: torch.Tensor, scales: torch.Tensor, out: torch.Tensor, positions: torch.Tensor,
+                         tok_seq: torch.Tensor, block_table: torch.Tensor, tok_index: torch.Tensor | None, window: int | None,
+                         scale: float, longest: int, gate: torch.Tensor | None = None, sink: bool = False) -> None:
+    """Causal attention of sequences that bring one token (``tok_index``: their rows of ``q`` [T, H, D], negative ones skipped;
+    None: every row is one, in order) over an 8-bit cache that holds this step's keys; writes those rows of ``out``. ``window``: as in
+    ``attention``. ``longest``: an upper bound of the positions any of the sequences holds, this token's included; it only picks how many ways
+    a row's keys are shared out. ``gate`` [T, H]: the per-head output gate, ``round(o) * round(sigmoid(gate))``; ``sink``: the
+    softmax's denominator has one term more, a key of score 0 without a value."""
+    name = "attention_kv8_decode"
+    shape = _check_attention(name, q, pool, scales, out, positions, tok_seq, block_table, gate)
+    _here(name, tok_index)
+    n = shape[0] if tok_index is None else ops._i32(tok_index, "tok_index").numel()
+    if n:
+        _attend(q, pool, scales, out, positions, tok_seq, block_table, tok_index, None, n, 1, shape, window, scale, longest, gate, sink)
+
+
+def attention_kv8_tokens(heads: int, kv_heads: int, head_dim: int, page: int, dtype: torch.dtype) -> int:
+    """The most tokens of one sequence that a tile of ``attention_kv8_prefill`` has."""
+    return _lib.call("tk_attn_kv8_tokens", heads, kv_heads)
+
+
+def attention_kv8_prefill(q: torch.Tensor, pool: torch.Tensor, scales: torch.Tensor, out: torch.Tensor, positions: torch.Tensor,
+                          tok_seq: torch.Tensor, block_table: torch.Tensor, tile_tok0: torch.Tensor, tile_ntok: torch.Tensor,
+                          window: int | None, scale: float, longest: int, gate: torch.Tensor | None = None,
+                          sink: bool = False) -> None:
+    """The same for prompt portions: tiles of at most ``attention_kv8_tokens`` tokens of one sequence at consecutive positions (``tile_tok0``:
+    each one's first row of ``q``; ``tile_ntok``: its tokens, 0 for an unused entry); writes the tiles' rows of ``out``."""
+    name = "attention_kv8_prefill"
+    shape = T, H, Hkv, P, D, code = _check_attention(name, q, pool, scales, out, positions, tok_seq, block_table, gate)
+    _here(name, tile_tok0, tile_ntok)
+    n = ops._i32(tile_tok0, "tile_tok0").numel()
+    if ops._i32(tile_ntok, "tile_ntok").numel() != n:
+        raise KernelError(f"{name}: {n} first tokens for {tile_ntok.numel()} tiles")
+    if n:
+        rows = _lib.call("tk_attn_kv8_tokens", H, Hkv)
+        _attend(q, pool, scales, out, positions, tok_seq, block_table, tile_tok0, tile_ntok, n, rows, shape, window, scale, longest, gate, sink)
+
+
+def copy_rows(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int]) -> None:
+    """``t[dst[i]] = t[src[i]]`` for every tensor ``t`` (contiguous, of any type) and every i, in one launch: pages of a cache's layers, or
+    requests' state rows. ``src`` and ``dst`` are host integers; no row is a destination twice, and none both a source and a
+    destination (refused)."""
+    _here("copy_rows", *tensors)
+    for t in tensors:
+        if t.dim() < 1 or not t.is_contiguous():
+            raise KernelError("copy_rows: contiguous tensors whose first dimension counts the rows")
+    if len(src) != len(dst):
+        raise KernelError(f"copy_rows: {len(src)} sources for {len(dst)} destinations")
+    tensors = [t for t in tensors if t.numel()]
+    if not tensors or not len(src):
+        return
+    try:
+        a, b = array.array("i", src), array.array("i", dst)
+    except (TypeError, OverflowError) as exc:
+        raise KernelError(f"copy_rows: rows are numbered by 32-bit integers ({exc})") from None
+    n = len(tensors)
+    base = (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors])
+    row = (ctypes.c_int64 * n)(*[t.stride(0) * t.element_size() if t.shape[0] > 1 else t.numel() * t.element_size() for t in tensors])
+    rows = (ctypes.c_int * n)(*[t.shape[0] for t in tensors])
+    _lib.call("tk_copy_rows", base, row, rows, n, a.buffer_info()[0], b.buffer_info()[0], len(a), ops._stream())
