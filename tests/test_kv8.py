@@ -371,7 +371,7 @@ def test_attention_with_peaked_scores_and_scales_far_apart(dtype):
     check_attention(Cache(lens, 1, 64, 16).fill(), [1, 65], 4, dtype, size=40.0)
     check_attention(Cache(lens, 1, 64, 16).fill(spread=30), [1, 65], 4, dtype)
     check_attention(Cache(lens, 1, 64, 16).fill(), [50, 1], 4, dtype, size=1e-12)
-    check_attention(Cache(lens, 1, 64, 16).fill(), [1, 1], 4, dtype, scale=0.0)
+    check_attention(Cache(lens, 1, 64, 16).fill(), [1, 1], 4, dtype, scale=1e-30)
 
 
 @gpu
@@ -611,6 +611,8 @@ def test_entry_points_refuse_shapes_that_are_not_built():
         assert not ops.kv8_supported(H, G, D)
         with pytest.raises(KernelError, match="not taken"):
             _lib.call("tk_attn_kv8", 256, 256, 256, 256, 256, 256, 256, 1, None, None, 1, H, G, D, 16, 0, 1.0, 1, None, None, 0, 0, 1, None)
+    with pytest.raises(KernelError, match="positive"):
+        _lib.call("tk_attn_kv8", 256, 256, 256, 256, 256, 256, 256, 1, None, None, 1, 4, 2, 64, 16, 0, 0.0, 1, None, None, 0, 0, 1, None)
     with pytest.raises(KernelError, match="bad sizes"):
         _lib.call("tk_attn_kv8", 256, 256, 256, 256, 256, 256, 256, 1, None, None, 1, 4, 2, 64, 16, 0, 1.0, 4, None, None, 0, 0, 1, None)
 

@@ -34,6 +34,14 @@ namespace {
 
 constexpr int K8_ROWS = 16;
 constexpr int K8_WARPS = 4, K8_THREADS = K8_WARPS * 32;
+#ifndef K8_MINB
+#define K8_MINB (D == 64 && sizeof(T) == 2 ? 4 : 2)
+#endif
+#ifndef K8_DEPTH_
+#define K8_DEPTH_ 3
+#endif
+constexpr int K8_DEPTH = K8_DEPTH_;                       // units of keys and values a warp has in shared memory or on their way
+constexpr long long K8_WAIT_CYCLES = 2000000000LL;
 constexpr float K8_LOG2E = 1.4426950408889634f;
 constexpr float K8_LAZY = 8.0f, K8_LIFT = 7.0f;
 
@@ -54,6 +62,36 @@ __device__ __forceinline__ float k8_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ int g_k8_error = 0;
+
+// Whether the barrier's phase completed; a wait ends after about a second, or once another thread has given up.
+__device__ __forceinline__ bool k8_try(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ bool k8_wait(uint32_t bar, uint32_t parity) {
+    if (k8_try(bar, parity)) return true;
+    const long long start = clock64();
+    int it = 0;
+    while (!k8_try(bar, parity)) {
+        if ((++it & 255) == 0) {
+            if (*(volatile int*)&g_k8_error != 0) return false;
+            if (clock64() - start > K8_WAIT_CYCLES) {
+                atomicCAS(&g_k8_error, 0, 1);
+                return false;
+            }
+        }
+    }
+    return true;
 }
 
 struct K8Args {
@@ -86,14 +124,15 @@ __device__ __forceinline__ float k8_gated(float o, const K8Args& a, int tok, int
 // T: type of q and the output. D: head size. PAGE16: pages are a multiple of 16 positions and a power of two, so 16 keys that begin at a multiple of
 // 16 lie in one page; otherwise every lane looks its own keys' pages up.
 template <typename T, int D, bool PAGE16>
-__global__ void __launch_bounds__(K8_THREADS)
+__global__ void __launch_bounds__(K8_THREADS, K8_MINB)
 attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, const K8Args a) {
     constexpr bool WIDE = sizeof(T) == 4;                // q and the weights as two float16
     constexpr int U = D == 64 ? 2 : 1;                   // groups of 16 keys a warp takes at a time
     constexpr int KS = D / 16, NT = D / 8;               // steps of q . k, column tiles of the output
     constexpr int KW = D / 64;                           // 16-byte words a lane reads of a key
     constexpr int VW = D / 32;                           // 4-byte words a lane reads of a value row
-    extern __shared__ float smem[];
+    constexpr int UNIT = U * 32 * D;                     // a unit's bytes
+    extern __shared__ __align__(128) float smem[];
     pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -108,9 +147,9 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
     const int lo = first_seen(pos_first, a.window), lo_last = first_seen(pos_last, a.window);
     // groups of 16 keys, from the one that holds `lo`; this CTA's are [g_begin, g_end), its warps take U of them in turn
     const int g_lo = lo >> 4, g_all = (pos_last >> 4) - g_lo + 1;
-    const int units = (g_all + U - 1) / U;
-    const int g_begin = g_lo + (int)((int64_t)units * split / a.nsplit) * U;
-    const int g_end = min(g_lo + (int)((int64_t)units * (split + 1) / a.nsplit) * U, g_lo + g_all);
+    const int all_units = (g_all + U - 1) / U;
+    const int g_begin = g_lo + (int)((int64_t)all_units * split / a.nsplit) * U;
+    const int g_end = min(g_lo + (int)((int64_t)all_units * (split + 1) / a.nsplit) * U, g_lo + g_all);
 
     // ---- q: rows g and g + 8, columns [c D / 4, (c + 1) D / 4) ----
     uint32_t qa[KS][4], qb[WIDE ? KS : 1][4];
@@ -154,68 +193,63 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
             }
     }
 
-    // ---- keys and values: the next groups' bytes and scales are on their way while these are used ----
+    // ---- where keys and values come from ----
     const int P = a.P;
-    const size_t head = (size_t)kvh * P * D, v_delta = (size_t)a.Hkv * P * D, page_bytes = 2 * v_delta;
-    uint4 kw[U][2][KW];
-    uint32_t vw[U][4][VW];
-    constexpr int NS = PAGE16 ? 1 : 4;                   // scales a group has for a lane: one, or one for each of its four keys
-    float ks_[U][NS], vs_[U][NS];
-    int page_next[U];
-    auto look_up = [&](int gr) {
-        if constexpr (PAGE16) {
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                page_next[u] = gr + u < g_end ? TK_PAGE(TK_K_KV8_ATTN, bt[((gr + u) << 4) >> a.p_shift]) : 0;
+    const size_t v_delta = (size_t)a.Hkv * P * D, page_bytes = 2 * v_delta;
+    const uint8_t* head = pool + (size_t)kvh * P * D;
+    const int units = (g_end - g_begin + U - 1) / U;
+    const int mine = units > warp ? (units - warp + K8_WARPS - 1) / K8_WARPS : 0;         // this warp's: unit warp, warp + K8_WARPS, ...
+    auto group_of = [&](int k, int u) { return g_begin + (warp + k * K8_WARPS) * U + u; };
+    // PAGE16: lane i knows the page and, from when its bytes are asked for, the scales of group i of a block of 32 groups
+    constexpr int BLOCK = 32 / U;
+    int page_now = 0, page_then = 0;
+    float sk_now = 1.f, sv_now = 1.f, sk_then = 1.f, sv_then = 1.f;
+    auto page_of_block = [&](int block) {
+        const int gr = group_of(block * BLOCK + lane / U, lane % U);
+        return gr < g_end ? TK_PAGE(TK_K_KV8_ATTN, bt[(gr << 4) >> a.p_shift]) : -1;
+    };
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + (uint32_t)warp * (K8_DEPTH * UNIT);
+    const uint32_t bars = (uint32_t)__cvta_generic_to_shared(smem) + K8_WARPS * K8_DEPTH * UNIT + (uint32_t)warp * (K8_DEPTH * 8);
+    const uint8_t* stage = reinterpret_cast<const uint8_t*>(smem) + warp * (K8_DEPTH * UNIT);
+    auto issue = [&](int k) {
+        if (k >= mine) return;
+        if (k % BLOCK == 0) {
+            page_now = k == 0 ? page_of_block(0) : page_then;
+            page_then = page_of_block(k / BLOCK + 1);
+            const float* sc = scales + (size_t)max(page_now, 0) * (2 * a.Hkv) + kvh;
+            sk_then = page_now >= 0 ? sc[0] : 1.f;
+            sv_then = page_now >= 0 ? sc[a.Hkv] : 1.f;
+        }
+        const int first = group_of(k, 0), n = min(U, g_end - first);
+        const uint32_t bar = bars + (uint32_t)(k % K8_DEPTH) * 8;
+        const int page = __shfl_sync(0xffffffffu, page_now, (k % BLOCK) * U + (lane >> 1) % U);
+        if (lane == 0)
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n * 32 * D) : "memory");
+        __syncwarp();
+        if (lane < 2 * n) {
+            const int u = lane >> 1, which = lane & 1;
+            const uint8_t* src = head + (size_t)page * page_bytes + which * v_delta + (uint32_t)((((first + u) << 4) & (P - 1)) * D);
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                             ring + (uint32_t)(k % K8_DEPTH) * UNIT + (uint32_t)(u * 32 * D + which * 16 * D)),
+                         "l"(src), "r"(16 * D), "r"(bar)
+                         : "memory");
         }
     };
-    auto load = [&](int gr) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int j0 = (gr + u) << 4;
-            const bool whole = gr + u < g_end;
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int j = j0 + 8 * t + g;
-                const bool there = whole && j >= lo && j <= pos_last;
-                const uint8_t* src = nullptr;
-                if (there) {
-                    const int page = PAGE16 ? page_next[u] : TK_PAGE(TK_K_KV8_ATTN, bt[j / P]);
-                    src = pool + (size_t)page * page_bytes + head + (size_t)(PAGE16 ? j & (P - 1) : j % P) * D + c * (D / 4);
-                }
-#pragma unroll
-                for (int w = 0; w < KW; ++w) kw[u][t][w] = there ? *reinterpret_cast<const uint4*>(src + 16 * w) : make_uint4(0u, 0u, 0u, 0u);
-            }
-            if constexpr (PAGE16) {
-                const float* s = scales + (size_t)page_next[u] * 2 * a.Hkv + kvh;
-                ks_[u][0] = whole ? s[0] : 1.f;
-                vs_[u][0] = whole ? s[a.Hkv] : 1.f;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int j = j0 + 2 * c + (i & 1) + 8 * (i >> 1);
-                const bool there = whole && j >= lo && j <= pos_last;
-                const uint8_t* src = nullptr;
-                int page = 0;
-                if (there) {
-                    page = PAGE16 ? page_next[u] : TK_PAGE(TK_K_KV8_ATTN, bt[j / P]);
-                    src = pool + (size_t)page * page_bytes + head + v_delta + (size_t)(PAGE16 ? j & (P - 1) : j % P) * D + g * (D / 8);
-                }
-                if constexpr (!PAGE16) {
-                    const float* s = scales + (size_t)page * 2 * a.Hkv + kvh;
-                    ks_[u][i] = there ? s[0] : 1.f;
-                    vs_[u][i] = there ? s[a.Hkv] : 1.f;
-                }
-                if constexpr (VW == 2) {
-                    const uint2 w = there ? *reinterpret_cast<const uint2*>(src) : make_uint2(0u, 0u);
-                    vw[u][i][0] = w.x, vw[u][i][1] = w.y;
-                } else {
-                    const uint4 w = there ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
-                    vw[u][i][0] = w.x, vw[u][i][1] = w.y, vw[u][i][2] = w.z, vw[u][i][3] = w.w;
-                }
-            }
+    if constexpr (PAGE16) {
+        if (lane == 0) {
+            for (int i = 0; i < K8_DEPTH; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bars + i * 8) : "memory");
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-    };
+        __syncwarp();
+        for (int k = 0; k < K8_DEPTH - 1; ++k) issue(k);
+    }
+    // A key's place among a group's 16: tile t, column n holds key 8 t + order(n); with it the value rows that the four lanes of a column read lie
+    // on both halves of the banks, and so do two neighbouring columns' keys.
+    auto order = [](int n) { return n ^ ((n >> 1) & 1); };
+    const int k_row = order(g), v_row0 = order(2 * c), v_row1 = order(2 * c + 1);
+    auto key_in_group = [&](int t, int e) { return 8 * t + (e ? v_row1 : v_row0); };       // of this lane's columns 2c + e
+    bool waited = true;
 
     float o[NT][4];
 #pragma unroll
@@ -223,16 +257,57 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    constexpr int STEP = K8_WARPS * U;
-    int gr = g_begin + warp * U;
-    if (gr < g_end) {
-        look_up(gr);
-        load(gr);
-        look_up(gr + STEP);
-    }
-    for (; gr < g_end; gr += STEP) {
-        // scores in base-2 logarithms with the value blocks' exponents in them: x[u][t] of keys 2c, 2c + 1 of tile t, rows g and g + 8
-        float x[U][2][4], inv_vs[U][NS];
+    for (int k = 0; k < mine; ++k) {
+        const int gr = group_of(k, 0);
+        const bool inner = (gr << 4) >= lo && ((gr + U) << 4) <= min(pos_last + 1, g_end << 4);      // all of its keys are read
+        const uint8_t* here = stage + (k % K8_DEPTH) * UNIT;
+        constexpr int NS = PAGE16 ? 1 : 4;               // scales a group has for a lane: one, or one for each of its four keys
+        float ksc[U][NS], vsc[U][NS];
+        uint4 kw[U][2][KW];
+        if constexpr (PAGE16) {
+            issue(k + K8_DEPTH - 1);
+            if (k % BLOCK == 0) {                        // (asked for when the first of the block's bytes were)
+                sk_now = sk_then;
+                sv_now = sv_then;
+            }
+            waited = waited && k8_wait(bars + (uint32_t)(k % K8_DEPTH) * 8, (uint32_t)((k / K8_DEPTH) & 1));
+            if (!__all_sync(0xffffffffu, waited)) break;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int w = 0; w < KW; ++w)
+                        kw[u][t][w] = *reinterpret_cast<const uint4*>(here + u * 32 * D + (8 * t + k_row) * D + c * (D / 4) + 16 * w);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int j = ((gr + u) << 4) + 8 * t + k_row;
+                    const bool there = gr + u < g_end && j >= lo && j <= pos_last;
+#pragma unroll
+                    for (int w = 0; w < KW; ++w) kw[u][t][w] = make_uint4(0u, 0u, 0u, 0u);
+                    if (there) {
+                        const uint8_t* src = head + (size_t)TK_PAGE(TK_K_KV8_ATTN, bt[j / P]) * page_bytes + (size_t)(j % P) * D + c * (D / 4);
+#pragma unroll
+                        for (int w = 0; w < KW; ++w) kw[u][t][w] = *reinterpret_cast<const uint4*>(src + 16 * w);
+                    }
+                }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = ((gr + u) << 4) + key_in_group(i >> 1, i & 1);
+                    const bool there = gr + u < g_end && j >= lo && j <= pos_last;
+                    const float* sc = scales + (size_t)(there ? TK_PAGE(TK_K_KV8_ATTN, bt[j / P]) : 0) * (2 * a.Hkv) + kvh;
+                    ksc[u][i] = there ? sc[0] : 1.f;
+                    vsc[u][i] = there ? sc[a.Hkv] : 1.f;
+                }
+        }
+        // products of keys 2c, 2c + 1 of tile t with rows g and g + 8; a key's logarithm is x * kc + ev, with the value block's exponent in it
+        float x[U][2][4], kc[U][NS][2], ev[U][NS], inv_vs[U][NS];
+        float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int u = 0; u < U; ++u) {
 #pragma unroll
@@ -248,47 +323,41 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
                     if constexpr (WIDE) mma_f16(x[u][t], qb[ks], b0, b1);
                 }
             }
-            float ksc[NS], ev[NS];
+            if constexpr (PAGE16) {
+                ksc[u][0] = __shfl_sync(0xffffffffu, sk_now, (k % BLOCK) * U + u);
+                vsc[u][0] = __shfl_sync(0xffffffffu, sv_now, (k % BLOCK) * U + u);
+            }
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
-                const int be = (__float_as_int(vs_[u][i]) >> 23) & 255;
-                ev[i] = (float)(be - 127);
-                inv_vs[u][i] = __int_as_float((254 - be) << 23);
-                ksc[i] = ks_[u][i];
+                // of a power of two: its exponent as a number, and its inverse
+                const int bits = __float_as_int(vsc[u][i]);
+                ev[u][i] = __int_as_float(0x4b000000 | (bits >> 23)) - 8388735.0f;
+                inv_vs[u][i] = __int_as_float((254 << 23) - bits);
+                // (never 0: what is hidden is minus infinity before it is multiplied)
+                kc[u][i][0] = fmaxf(ksc[u][i] * row_c[0], 1.2e-38f);
+                kc[u][i][1] = fmaxf(ksc[u][i] * row_c[1], 1.2e-38f);
             }
             const int j0 = (gr + u) << 4;
-            const bool masked = j0 + 15 > pos_first || j0 < lo_last || gr + u >= g_end;
+            if (j0 + 15 > pos_first || j0 < lo_last || gr + u >= g_end) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int i = PAGE16 ? 0 : 2 * t + (e & 1);
-                    x[u][t][e] = fmaf(x[u][t][e], ksc[i] * row_c[e >> 1], ev[i]);
-                    if (masked) {
-                        const int j = j0 + 8 * t + 2 * c + (e & 1), p = row_pos[e >> 1];
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = j0 + key_in_group(t, e & 1), p = row_pos[e >> 1];
                         if (j > p || j < first_seen(p, a.window) || gr + u >= g_end) x[u][t][e] = -INFINITY;
                     }
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                if constexpr (PAGE16) {
+                    const float most = fmaxf(fmaxf(x[u][0][2 * r], x[u][0][2 * r + 1]), fmaxf(x[u][1][2 * r], x[u][1][2 * r + 1]));
+                    top[r] = fmaxf(top[r], fmaf(most, kc[u][0][r], ev[u][0]));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top[r] = fmaxf(top[r], fmaf(x[u][i >> 1][2 * r + (i & 1)], kc[u][i][r], ev[u][i]));
                 }
+            }
         }
-        // the values' bytes leave their registers before the next groups' arrive
-        uint32_t vc[U][4][VW];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int w = 0; w < VW; ++w) vc[u][i][w] = vw[u][i][w];
-        if (gr + STEP < g_end) {
-            load(gr + STEP);
-            look_up(gr + 2 * STEP);
-        }
-        float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], x[u][t][e]);
         if (__any_sync(0xffffffffu, top[0] > m[0] + K8_LAZY || top[1] > m[1] + K8_LAZY)) {
 #pragma unroll
             for (int hrow = 0; hrow < 2; ++hrow) {
@@ -313,21 +382,42 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int hrow = 0; hrow < 2; ++hrow) {
-                    const float w0 = k8_exp2(x[u][t][2 * hrow] + base[hrow]), w1 = k8_exp2(x[u][t][2 * hrow + 1] + base[hrow]);
-                    l[hrow] = fmaf(w0, inv_vs[u][PAGE16 ? 0 : 2 * t], l[hrow]);
-                    l[hrow] = fmaf(w1, inv_vs[u][PAGE16 ? 0 : 2 * t + 1], l[hrow]);
+                    const int i0 = PAGE16 ? 0 : 2 * t, i1 = PAGE16 ? 0 : 2 * t + 1;
+                    const float w0 = k8_exp2(fmaf(x[u][t][2 * hrow], kc[u][i0][hrow], ev[u][i0] + base[hrow]));
+                    const float w1 = k8_exp2(fmaf(x[u][t][2 * hrow + 1], kc[u][i1][hrow], ev[u][i1] + base[hrow]));
+                    l[hrow] = fmaf(w0, inv_vs[u][i0], l[hrow]);
+                    l[hrow] = fmaf(w1, inv_vs[u][i1], l[hrow]);
                     pa[hrow + 2 * t] = half2_bits(w0, w1);
                     if constexpr (WIDE) {
                         const float2 hi = half2_floats(pa[hrow + 2 * t]);
                         pb[hrow + 2 * t] = half2_bits(w0 - hi.x, w1 - hi.y);
                     }
                 }
+            uint32_t vw[4][VW];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = key_in_group(i >> 1, i & 1), j = ((gr + u) << 4) + row;
+                const bool there = inner || (gr + u < g_end && j >= lo && j <= pos_last);
+                const uint8_t* src = here + u * 32 * D + 16 * D + row * D + g * (D / 8);
+                if constexpr (!PAGE16)
+                    if (there) src = head + (size_t)TK_PAGE(TK_K_KV8_ATTN, bt[j / P]) * page_bytes + v_delta + (size_t)(j % P) * D + g * (D / 8);
+                // (what is not to be read is in shared memory all the same where a page's bytes came as one, and never matters)
+                if constexpr (VW == 2) {
+                    uint2 v = make_uint2(0u, 0u);
+                    if (there) v = *reinterpret_cast<const uint2*>(src);
+                    vw[i][0] = v.x, vw[i][1] = v.y;
+                } else {
+                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                    if (there) v = *reinterpret_cast<const uint4*>(src);
+                    vw[i][0] = v.x, vw[i][1] = v.y, vw[i][2] = v.z, vw[i][3] = v.w;
+                }
+            }
 #pragma unroll
             for (int w = 0; w < VW; ++w)
 #pragma unroll
                 for (int pair = 0; pair < 2; ++pair) {
                     const uint32_t sel = pair ? 0x7362 : 0x5140;
-                    const uint32_t y0 = __byte_perm(vc[u][0][w], vc[u][1][w], sel), y1 = __byte_perm(vc[u][2][w], vc[u][3][w], sel);
+                    const uint32_t y0 = __byte_perm(vw[0][w], vw[1][w], sel), y1 = __byte_perm(vw[2][w], vw[3][w], sel);
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const int j = 4 * w + 2 * pair + e;
@@ -346,6 +436,7 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
         m[hrow] = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
     }
 
+    __syncthreads();                                     // (the ring's place is used again)
     // ---- the warps' shares joined: [warp][row] D floats (4 apart from a power of two) and [warp][row] (m, l) ----
     constexpr int LD = D + 4;
     float* share = smem;
@@ -431,8 +522,13 @@ attn_kv8_merge_kernel(T* out, const K8Args a) {
 
 template <typename T, int D, bool PAGE16>
 cudaError_t k8_launch(const void* q, const void* pool, const float* scales, void* out, const K8Args& a, cudaStream_t stream) {
-    constexpr int smem = (K8_WARPS * K8_ROWS * (D + 4) + 2 * K8_WARPS * K8_ROWS) * 4;
-    static_assert(smem <= 48 * 1024, "within what a kernel has without asking");
+    constexpr int shares = (K8_WARPS * K8_ROWS * (D + 4) + 2 * K8_WARPS * K8_ROWS) * 4;
+    constexpr int ring = PAGE16 ? K8_WARPS * K8_DEPTH * (4096 + 8) : 0;
+    constexpr int smem = ring > shares ? ring : shares;
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(attn_kv8_kernel<T, D, PAGE16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+    }
     return tk_launch(attn_kv8_kernel<T, D, PAGE16>, dim3((unsigned)(a.items * a.Hkv * a.nsplit)), dim3(K8_THREADS), smem, stream, (const T*)q,
                      (const uint8_t*)pool, scales, (T*)out, a);
 }
@@ -467,6 +563,14 @@ TK_API int tk_attn_kv8_splits(int items, int Hkv, int longest, int sm_count) {
     return (int)(n < 1 ? 1 : n > 128 ? 128 : n);
 }
 
+// 0, or 1 if a warp gave up waiting for its keys since the last call. Resets the word.
+TK_API int tk_attn_kv8_status() {
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_k8_error, sizeof(int)) != cudaSuccess) return -1;
+    if (v != 0) cudaMemcpyToSymbol(g_k8_error, &zero, sizeof(int));
+    return v;
+}
+
 // q, out: [T, H, D]; pool: [pages, 2, Hkv, P, D] bytes, scales: [pages, 2, Hkv]. item_tok0 / item_ntok: tiles of at most tk_attn_kv8_tokens tokens of one
 // sequence at consecutive positions (0 tokens: skipped); item_ntok null: single tokens' rows (negative: skipped; item_tok0 null too: rows 0, 1, ...).
 // window: see first_seen. scratch: items * H * (tokens a tile, or 1) * nsplit * (D + 4) floats when nsplit > 1. gate: [T, >= H], the per-head output gate.
@@ -479,6 +583,7 @@ TK_API int tk_attn_kv8(const void* q, const void* pool, const float* scales, voi
     TK_CHECK_ARG(items >= 0 && P > 0 && nsplit >= 1 && (nsplit == 1 || scratch != nullptr), "attn_kv8: bad sizes");
     TK_CHECK_ARG(item_ntok == nullptr || item_tok0 != nullptr, "attn_kv8: tiles have first tokens");
     TK_CHECK_ARG((int64_t)items * Hkv * nsplit < 0x7fffffff, "attn_kv8: %d splits of %d items", nsplit, items);
+    TK_CHECK_ARG(scale > 0.f, "attn_kv8: the scores' factor is positive");
     TK_CHECK_ARG(dtype == TK_F32 || dtype == TK_BF16, "attn_kv8: unknown dtype %d", dtype);
     TK_CHECK_ARG((uintptr_t)q % 16 == 0 && (uintptr_t)pool % 16 == 0 && (uintptr_t)out % 16 == 0, "attn_kv8: 16-byte aligned tensors");
     if (items == 0) return 0;

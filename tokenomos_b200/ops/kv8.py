@@ -161,6 +161,11 @@ def attention_kv8_prefill(q: torch.Tensor, pool: torch.Tensor, scales: torch.Ten
         _attend(q, pool, scales, out, positions, tok_seq, block_table, tile_tok0, tile_ntok, n, rows, shape, window, scale, longest, gate, sink)
 
 
+def attention_kv8_status() -> int:
+    """0, or where a warp of the 8-bit cache's attention gave up waiting for its keys since the last call."""
+    return _lib.call("tk_attn_kv8_status")
+
+
 def copy_rows(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int]) -> None:
     """``t[dst[i]] = t[src[i]]`` for every tensor ``t`` (contiguous, of any type) and every i, in one launch: pages of a cache's layers, or
     requests' state rows. ``src`` and ``dst`` are host integers; no row is a destination twice, and none both a source and a
