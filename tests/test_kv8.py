@@ -40,9 +40,9 @@ def norm_rope(x, w, eps, freq, pos, mult, interleaved):
     return out
 
 
-def attend(q, kv, pos, window, scale, sink=False):
-    """q [T, H, D], kv [2, G, L, D] (float64, one sequence's cache), pos [T]: (outputs, sum of p |v| per output, largest |score| and sum
-    |q k| scale per row), the last ones for the bounds."""
+def attend(q, kv, pos, window, scale, sv, sink=False):
+    """q [T, H, D], kv [2, G, L, D] (float64, one sequence's cache), pos [T], sv [G, L] (the values' scales): (outputs, sum of p |v| per output,
+    and for the bounds the largest sum |q k| scale of a row and what 8-bit terms leave)."""
     T, H, D = q.shape
     G, L = kv.shape[1], kv.shape[2]
     k, v = kv.repeat_interleave(H // G, 1)
@@ -61,19 +61,31 @@ def attend(q, kv, pos, window, scale, sink=False):
     seen_v = torch.where(see.any(0)[None, :, None], v, 0.0)
     o = torch.einsum("htl,hld->thd", p, seen_v)
     size = torch.einsum("htl,hld->thd", p, seen_v.abs())
-    reach = torch.einsum("thd,hld->htl", q.abs(), torch.where(see.any(0)[None, :, None], k, 0.0).abs()).amax(-1).t() * abs(scale)
-    return o, size, reach
+    seen_k = torch.where(see.any(0)[None, :, None], k, 0.0).abs()
+    reach = torch.einsum("thd,hld->htl", q.abs(), seen_k).amax(-1).t() * abs(scale)
+    # what the terms of q and of the weights leave: 2^-18 of q's largest element beside every key element; 2^-24 of the row's largest weight of a
+    # value's byte beside every byte
+    left = q.abs().amax(-1) * seen_k.sum(-1).amax(-1)[None] * abs(scale) * 2.0 ** -18
+    sv = sv.double().repeat_interleave(H // G, 0)
+    rest = (p * sv[:, None]).amax(-1).t()[..., None] * (seen_v.abs() / sv[..., None]).sum(1)[None] * 2.0 ** -24
+    return o, size, (reach, left, rest)
 
 
 def within(got, want, size, reach, keys, dtype):
     """The kernel's bound. A weight's relative error: its score (D products in 32-bit sums, a few roundings of a number of at most
     `reach` log2(e): (D + 8) 2^-24 of it, and for 32-bit q 2^-22 from its two halves), the exponential's 2^-22, its rounding to
-    float16 (2^-11; as two float16 2^-22); the same for the sum; sums over keys in 32 bits; one rounding of the result."""
+    float16 (2^-11; as two float16 2^-22; as four e4m3 terms 2^-16) and, in terms, what they leave (``attend``); the same for the sum; sums over
+    keys in 32 bits, each term's products their own; one rounding of the result."""
     D = want.shape[-1]
     unit = torch.finfo(dtype).eps / 2
-    eps = reach[..., None] * ((D + 8) * 2.0 ** -24 + (2.0 ** -22 if dtype == torch.float32 else 0)) + 2.0 ** -22
-    half = 2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -22
-    bound = unit * want.abs() * 1.01 + size * (2 * eps + half + 2 * (keys + 64) * 2.0 ** -24) + 2.0 ** -120
+    reach, left, rest = reach
+    eps = reach[..., None] * ((2 * D + 8) * 2.0 ** -24 + (2.0 ** -22 if dtype == torch.float32 else 0)) + 2.0 ** -22
+    half = 2.0 ** -22
+    if dtype == torch.bfloat16:
+        eps, half = eps + left[..., None], 2.0 ** -11
+    bound = unit * want.abs() * 1.01 + size * (2 * eps + half + 8 * (keys + 64) * 2.0 ** -24) + 2.0 ** -120
+    if dtype == torch.bfloat16:
+        bound = bound + rest
     off = (got.double() - want).abs()
     assert torch.isfinite(got).all()
     assert (off <= bound).all(), ((off / bound).max().item(), off.max().item())
@@ -116,6 +128,12 @@ class Cache:
         rows = self.table[s, :-(-n // self.P)].long().cuda()
         raw = self.pool.view(torch.uint8)[rows].view(F8).double() * self.scales[rows].double()[..., None, None]
         return raw.permute(1, 2, 0, 3, 4).reshape(2, self.G, -1, self.D)[:, :, :n]
+
+
+    def value_scales(self, s, upto=None):
+        """[G, n]: of each position of sequence s."""
+        n = self.lens[s] if upto is None else upto
+        return self.scales[self.table[s, :-(-n // self.P)].long().cuda(), 1].t().repeat_interleave(self.P, 1)[:, :n]
 
 
 def i32(x):
@@ -319,7 +337,7 @@ def check_attention(cache, new, H, dtype, window=None, scale=None, sink=False, s
     out, pos = run_attention(cache, q, new, window, scale, sink=sink)
     start = 0
     for s, n in enumerate(new):
-        want, sz, reach = attend(q[start:start + n].double(), cache.of(s), pos[start:start + n], window, scale, sink)
+        want, sz, reach = attend(q[start:start + n].double(), cache.of(s), pos[start:start + n], window, scale, cache.value_scales(s), sink)
         within(out[start:start + n], want, sz, reach, cache.lens[s], dtype)
         start += n
 
@@ -372,6 +390,28 @@ def test_attention_with_peaked_scores_and_scales_far_apart(dtype):
     check_attention(Cache(lens, 1, 64, 16).fill(spread=30), [1, 65], 4, dtype)
     check_attention(Cache(lens, 1, 64, 16).fill(), [50, 1], 4, dtype, size=1e-12)
     check_attention(Cache(lens, 1, 64, 16).fill(), [1, 1], 4, dtype, scale=1e-30)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_small_weights_beside_a_large_one(dtype):
+    """The first key takes half of the weight and its value is 0: what comes out is the other thousands' (each about 2^-13 of it)."""
+    n = 8000
+    cache = Cache([n], 1, 64, 16).fill()
+    page, page1 = int(cache.table[0, 0]), cache.table[0, 1:].long().cuda()
+    cache.pool[page, :, :, 0] = torch.zeros(64, device="cuda").to(F8)
+    cache.pool[page, 0, 0, 0, 0] = torch.tensor(256.0).to(F8)
+    cache.scales[:] = 2.0 ** -7
+    q = torch.zeros(1, 4, 64, device="cuda", dtype=dtype)
+    q[0, :, 0] = 4.0
+    cache.pool.view(torch.uint8)[page1, 0, :, :, 0] = 0
+    cache.pool.view(torch.uint8)[page, 0, :, 1:, 0] = 0
+    scale = math.log(n) / (4.0 * 2.0)
+    out, pos = run_attention(cache, q, [1], None, scale)
+    want, sz, reach = attend(q.double(), cache.of(0), pos, None, scale, cache.value_scales(0))
+    within(out, want, sz, reach, n, dtype)
+    # (a tenth of the weights lost would move the mean of 8,000 random values by about as much)
+    assert ((out.double() - want).norm() / want.norm()).item() < 0.01
 
 
 @gpu
@@ -472,7 +512,7 @@ def test_a_run_of_steps_as_a_model_makes_them(dtype):
         start = 0
         for k, s in enumerate(live):
             n = step[s]
-            want, sz, reach = attend(q[start:start + n].double(), view.of(k), pos[start:start + n], None, D ** -0.5)
+            want, sz, reach = attend(q[start:start + n].double(), view.of(k), pos[start:start + n], None, D ** -0.5, view.value_scales(k))
             within(out[start:start + n], want, sz, reach, have[s], dtype)
             start += n
 
@@ -507,7 +547,7 @@ def test_two_recorded_calls_share_no_workspace_and_replay_on_new_contents():
     torch.cuda.synchronize()
     for k in (0, 1):
         for s, p in enumerate((700, 1400)):
-            want, sz, reach = attend(q[k][s:s + 1].double(), caches[k].of(s, p + 1), pos[s:s + 1], None, 0.125)
+            want, sz, reach = attend(q[k][s:s + 1].double(), caches[k].of(s, p + 1), pos[s:s + 1], None, 0.125, caches[k].value_scales(s, p + 1))
             within(out[k][s:s + 1], want, sz, reach, p + 1, torch.bfloat16)
 
 

@@ -28,21 +28,13 @@
 
 #include <type_traits>
 
-#include "kv8.cuh"
+#include "kv8_attn.cuh"
 
 namespace {
 
 constexpr int K8_ROWS = 16;
 constexpr int K8_WARPS = 4, K8_THREADS = K8_WARPS * 32;
-#ifndef K8_MINB
-#define K8_MINB (D == 64 && sizeof(T) == 2 ? 4 : 2)
-#endif
-#ifndef K8_DEPTH_
-#define K8_DEPTH_ 3
-#endif
-constexpr int K8_DEPTH = K8_DEPTH_;                       // units of keys and values a warp has in shared memory or on their way
-constexpr long long K8_WAIT_CYCLES = 2000000000LL;
-constexpr float K8_LOG2E = 1.4426950408889634f;
+constexpr int K8_DEPTH = 3;                       // units of keys and values a warp has in shared memory or on their way
 constexpr float K8_LAZY = 8.0f, K8_LIFT = 7.0f;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -56,75 +48,10 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float2 half2_floats(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
-
-__device__ __forceinline__ float k8_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ int g_k8_error = 0;
-
-// Whether the barrier's phase completed; a wait ends after about a second, or once another thread has given up.
-__device__ __forceinline__ bool k8_try(uint32_t bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.b32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-__device__ __forceinline__ bool k8_wait(uint32_t bar, uint32_t parity) {
-    if (k8_try(bar, parity)) return true;
-    const long long start = clock64();
-    int it = 0;
-    while (!k8_try(bar, parity)) {
-        if ((++it & 255) == 0) {
-            if (*(volatile int*)&g_k8_error != 0) return false;
-            if (clock64() - start > K8_WAIT_CYCLES) {
-                atomicCAS(&g_k8_error, 0, 1);
-                return false;
-            }
-        }
-    }
-    return true;
-}
-
-struct K8Args {
-    const int* positions;
-    const int* tok_seq;
-    const int* block_table;
-    const int* item_tok0;        // tiles' first tokens, or rows of single tokens (null: item i is row i)
-    const int* item_ntok;        // tiles' tokens (null: one each)
-    const void* gate;
-    float* scratch;              // [item, KV head, split, row] D + 2 floats, when nsplit > 1
-    int64_t ldg;
-    int bt_stride, items, H, Hkv, P, p_shift, window, nsplit, sink, rows_most;
-    float scale;
-};
-
-// The share of a row's keys that one CTA or warp has seen, under reference m: o = sum w v, l = sum w / s_V.
-__device__ __forceinline__ float k8_factor(float m, float l, float m_all) {
-    // (nothing seen: left out; a sum that is not a number under no maximum: every score was one)
-    return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : k8_exp2(m - m_all);
-}
-
-template <typename T>
-__device__ __forceinline__ float k8_gated(float o, const K8Args& a, int tok, int head) {
-    o = round_as<T>(o);
-    if (a.gate == nullptr) return o;
-    const float g = to_f<T>(reinterpret_cast<const T*>(a.gate)[(size_t)tok * a.ldg + head]);
-    return o * round_as<T>(1.0f / (1.0f + expf(-g)));
-}
-
 // T: type of q and the output. D: head size. PAGE16: pages are a multiple of 16 positions and a power of two, so 16 keys that begin at a multiple of
 // 16 lie in one page; otherwise every lane looks its own keys' pages up.
 template <typename T, int D, bool PAGE16>
-__global__ void __launch_bounds__(K8_THREADS, K8_MINB)
+__global__ void __launch_bounds__(K8_THREADS, D == 64 && sizeof(T) == 2 && PAGE16 ? 4 : 2)
 attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, const K8Args a) {
     constexpr bool WIDE = sizeof(T) == 4;                // q and the weights as two float16
     constexpr int U = D == 64 ? 2 : 1;                   // groups of 16 keys a warp takes at a time
@@ -471,8 +398,9 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
             if (a.sink && m_all > -INFINITY) l_all += k8_exp2(K8_LIFT - m_all);
             const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
             float4 y;
-            y.x = k8_gated<T>(v[0] * inv, a, tok, hd), y.y = k8_gated<T>(v[1] * inv, a, tok, hd);
-            y.z = k8_gated<T>(v[2] * inv, a, tok, hd), y.w = k8_gated<T>(v[3] * inv, a, tok, hd);
+            const float gate = k8_gate<T>(a, tok, hd);
+            y.x = k8_apply<T>(v[0] * inv, a, gate), y.y = k8_apply<T>(v[1] * inv, a, gate);
+            y.z = k8_apply<T>(v[2] * inv, a, gate), y.w = k8_apply<T>(v[3] * inv, a, gate);
             Quad<T>::store(out + ((size_t)tok * a.H + hd) * D + col, y);
         } else {
             float* part = a.scratch + ((((size_t)item * a.Hkv + kvh) * a.nsplit + split) * a.rows_most + r) * (D + 4);
@@ -480,44 +408,6 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
             if (col == 0) *reinterpret_cast<float2*>(part + D) = make_float2(m_all, l_all);
         }
     }
-}
-
-// The CTAs' shares of a row joined: a warp a row, D / 32 columns a lane.
-template <typename T, int D>
-__global__ void __launch_bounds__(128)
-attn_kv8_merge_kernel(T* out, const K8Args a) {
-    constexpr int C = D / 32;
-    pdl_launch_dependents();
-    pdl_wait();
-    const int lane = threadIdx.x & 31, G = a.H / a.Hkv;
-    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int r = (int)(at % a.rows_most), kvh = (int)(at / a.rows_most % a.Hkv);
-    const int64_t item = at / ((int64_t)a.rows_most * a.Hkv);
-    if (item >= a.items) return;
-    const int tok0 = a.item_tok0 != nullptr ? a.item_tok0[item] : (int)item;
-    const int ntok = a.item_ntok != nullptr ? a.item_ntok[item] : 1;
-    if (tok0 < 0 || r >= ntok * G) return;
-    const float* part = a.scratch + ((item * a.Hkv + kvh) * a.nsplit * a.rows_most + r) * (D + 4);
-    const size_t step = (size_t)a.rows_most * (D + 4);
-    float m_all = -INFINITY;
-    for (int s = lane; s < a.nsplit; s += 32) m_all = fmaxf(m_all, part[s * step + D]);
-    m_all = warp_max(m_all);
-    float v[C], l_all = 0.f;
-#pragma unroll
-    for (int e = 0; e < C; ++e) v[e] = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < a.nsplit; ++s) {
-        const float2 ml = *reinterpret_cast<const float2*>(part + s * step + D);
-        const float f = k8_factor(ml.x, ml.y, m_all);
-        l_all = fmaf(ml.y, f, l_all);
-#pragma unroll
-        for (int e = 0; e < C; ++e) v[e] = fmaf(part[s * step + lane * C + e], f, v[e]);
-    }
-    if (a.sink && m_all > -INFINITY) l_all += k8_exp2(K8_LIFT - m_all);
-    const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
-    const int tok = tok0 + r / G, hd = kvh * G + r % G;
-#pragma unroll
-    for (int e = 0; e < C; ++e) out[((size_t)tok * a.H + hd) * D + lane * C + e] = from_f<T>(k8_gated<T>(v[e] * inv, a, tok, hd));
 }
 
 template <typename T, int D, bool PAGE16>
@@ -540,8 +430,8 @@ cudaError_t k8_dispatch(const void* q, const void* pool, const float* scales, vo
                             : (page16 ? k8_launch<T, 128, true>(q, pool, scales, out, a, stream) : k8_launch<T, 128, false>(q, pool, scales, out, a, stream));
     if (e != cudaSuccess || a.nsplit == 1) return e;
     const unsigned grid = (unsigned)(((int64_t)a.items * a.Hkv * a.rows_most + 3) / 4);
-    return D == 64 ? tk_launch(attn_kv8_merge_kernel<T, 64>, dim3(grid), dim3(128), 0, stream, (T*)out, a)
-                   : tk_launch(attn_kv8_merge_kernel<T, 128>, dim3(grid), dim3(128), 0, stream, (T*)out, a);
+    return D == 64 ? tk_launch(attn_kv8_merge_kernel<T, 64>, dim3(grid), dim3(128), 0, stream, (T*)out, a, K8_LIFT)
+                   : tk_launch(attn_kv8_merge_kernel<T, 128>, dim3(grid), dim3(128), 0, stream, (T*)out, a, K8_LIFT);
 }
 
 }  // namespace
@@ -563,12 +453,16 @@ TK_API int tk_attn_kv8_splits(int items, int Hkv, int longest, int sm_count) {
     return (int)(n < 1 ? 1 : n > 128 ? 128 : n);
 }
 
+int tk_attn_kv8_tc(const void* q, const void* pool, const float* scales, void* out, const void* args, int D, cudaStream_t stream);
+int tk_attn_kv8_tc_status();
+
 // 0, or 1 if a warp gave up waiting for its keys since the last call. Resets the word.
 TK_API int tk_attn_kv8_status() {
     int v = 0, zero = 0;
     if (cudaMemcpyFromSymbol(&v, g_k8_error, sizeof(int)) != cudaSuccess) return -1;
     if (v != 0) cudaMemcpyToSymbol(g_k8_error, &zero, sizeof(int));
-    return v;
+    const int tc = tk_attn_kv8_tc_status();
+    return v != 0 ? v : tc;
 }
 
 // q, out: [T, H, D]; pool: [pages, 2, Hkv, P, D] bytes, scales: [pages, 2, Hkv]. item_tok0 / item_ntok: tiles of at most tk_attn_kv8_tokens tokens of one
@@ -593,6 +487,8 @@ TK_API int tk_attn_kv8(const void* q, const void* pool, const float* scales, voi
     const int G = H / Hkv;
     K8Args a{positions, tok_seq, block_table, item_tok0, item_ntok, gate, scratch, ldg, bt_stride, items, H, Hkv, P, shift, window, nsplit, sink,
              item_ntok != nullptr ? (K8_ROWS / G) * G : G, scale};
+    // single tokens of 16-bit models whose pages a tensor map can follow
+    if (dtype == TK_BF16 && item_ntok == nullptr && shift >= 4) return tk_attn_kv8_tc(q, pool, scales, out, &a, D, stream);
     const cudaError_t e = dtype == TK_F32 ? k8_dispatch<float>(q, pool, scales, out, a, D, stream)
                                           : k8_dispatch<__nv_bfloat16>(q, pool, scales, out, a, D, stream);
     if (e != cudaSuccess) {
