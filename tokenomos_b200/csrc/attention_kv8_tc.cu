@@ -1,22 +1,24 @@
 // Single tokens' attention over the 8-bit cache (kv8.cuh) on the fifth-generation tensor cores, for bfloat16: the cache's bytes are the products'
 // operands as they lie in memory, no instruction ever touches them.
 //
-//   S^T = K q^T      tcgen05.mma kind::f8f6f4, M = 128 keys, N = 16 query heads: a thread owns a key and reads its scores, a column a head
-//   O  += P V        M = 2 x 16 rows of 128 (the others hold whatever lies behind them in shared memory, and nobody reads their sums), N = D
+//   S^T = K q^T      tcgen05.mma kind::f8f6f4, M = 128 keys, a column a query head: a thread owns a key and reads its scores
+//   O^T += V^T P^T   M = D, the same columns: V's [key][d] is the M-major operand as it lands
 //
-// What is not 8-bit is a sum of 8-bit terms, multiplied one after the other into the same 32-bit accumulator: e4m3 has four significant bits, so q (after
+// What is not 8-bit is a sum of 8-bit terms, a column each, added up when they are read: e4m3 has four significant bits, so q (after
 // division by a power of two that brings its row's largest to [128, 256)) is two terms, exactly for elements down to 2^-12 of the row's
 // largest and to 2^-18 of that below. A weight is four: two that leave 2^-8 of it or 2^-10 (e4m3's smallest steps), and two of what they leave times
-// 2^8, in rows of their own (16 to 31) whose sums are added up divided by 2^8 at the end. The weights' reference maximum follows lazily (raised when
-// a row exceeds it by 2^2) and weights are lifted by 2^6 (at most 256, of 448): a weight is off by at most 2^-16 of itself or 2^-24 of
-// the row's largest. (One pair of terms alone loses the many small weights beside a large one: 30,000 keys that share half of a row's
-// weight with one that has the other half would be off by a tenth.) A value block's scale is in the exponent, as in attention_kv8.cu.
+// 2^8. The weights' reference maximum follows lazily (raised when a row exceeds it by 2^2) and weights are lifted by 2^6 (at most 256, of 448): a
+// weight is off by at most 2^-16 of itself or 2^-24 of the row's largest. (Two terms alone lose the many small weights beside a large one: 30,000
+// keys that share half of a row's weight with one that has the other half would be off by a tenth.) A value block's scale is in the
+// exponent, as in attention_kv8.cu. Columns cost nothing here: a product's time is that of reading its 128 x 32 or D x 32 bytes of the first operand
+// from shared memory. (With the heads as the M side of the second product, 32 rows of 128, and the terms one after the other, the products
+// alone took 575 cycles a tile of 128 keys, and 8 tokens behind 32,000 positions 71 us.)
 //
 // A CTA takes the query heads of one KV head of one token and a share of its keys, in tiles of 128:
 //   warp 4      brings K and V by TMA, a page (or 128 positions of one) a load, two or three tiles ahead
 //   warp 5      issues the products
 //   warps 0-3   thread = key: masks, reference maximum (one vote of the four warps a tile), weights, their terms into shared memory
-//               ([head][key], the first product operand of O); positions that are not to be seen have their value rows zeroed there
+//               ([term and head][key], the second product's other operand); positions that are not to be seen have their value rows zeroed there
 //
 // Masking and sums are those of attention_kv8.cu; every wait is bounded (about a second), the kernel then frees its tensor memory and
 // returns, and tk_attn_kv8_status() says so.
@@ -30,8 +32,7 @@ namespace {
 
 constexpr int K8T_KEYS = 128, K8T_ROWS = 16;
 constexpr int K8T_THREADS = 192;
-constexpr int K8T_QTERMS = 2, K8T_PTERMS = 2;
-constexpr int K8T_P_BYTES = 2 * K8T_ROWS * K8T_KEYS;      // of a term: [16 and 16 finer][128], 128-byte swizzle
+constexpr int K8T_QTERMS = 2, K8T_PTERMS = 4;
 constexpr float K8T_LAZY = 2.0f, K8T_LIFT = 6.0f, K8T_FINE = 256.0f;
 
 // K-major or MN-major operand whose rows are D = 64 (64-byte swizzle) or 128 bytes (128-byte swizzle), groups of eight rows one after the other
@@ -51,9 +52,9 @@ __device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
     return (uint32_t)(row * BYTES + ((BYTES == 64 ? chunk ^ ((row >> 1) & 3) : chunk ^ (row & 7)) << 4));
 }
 
-// e4m3 x e4m3 -> f32, M = 128
-__host__ __device__ constexpr uint32_t idesc8(int n, bool b_mn_major) {
-    return (1u << 4) | (b_mn_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+// e4m3 x e4m3 -> f32
+__host__ __device__ constexpr uint32_t idesc8(int m, int n, bool a_m_major) {
+    return (1u << 4) | (a_m_major ? 1u << 15 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
 __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -75,24 +76,29 @@ __device__ __forceinline__ bool elect_lane() {
     return mine != 0;
 }
 
-// N columns of this thread's lane
+// eight columns of this thread's lane; the loads of several calls are waited for together
+__device__ __forceinline__ void tmem_ld8_start(uint32_t addr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr));
+}
 template <int N>
 __device__ __forceinline__ void tmem_ld_n(uint32_t addr, float (&v)[N]) {
     uint32_t r[N];
-    if constexpr (N == 2)
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr));
-    else if constexpr (N == 4)
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-    else if constexpr (N == 8) {
-        tmem_ld8(addr, v);
-        return;
-    } else {
-        tmem_ld16(addr, v);
-        return;
-    }
+#pragma unroll
+    for (int i = 0; i < N; i += 8) tmem_ld8_start(addr + i, r + i);
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r[i]);
+}
+template <int N>
+__device__ __forceinline__ void tmem_st_n(uint32_t addr, const float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 8)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr + i), "f"(v[i]), "f"(v[i + 1]),
+                     "f"(v[i + 2]), "f"(v[i + 3]), "f"(v[i + 4]), "f"(v[i + 5]), "f"(v[i + 6]), "f"(v[i + 7])
+                     : "memory");
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
 // whether `mine` holds for any of the 128 threads of the weights' warps
@@ -114,18 +120,19 @@ __device__ __forceinline__ void sync_128() { asm volatile("bar.sync 2, 128;" :::
 template <int D>
 constexpr int k8t_stages = D == 64 ? 3 : 2;
 
-template <int D>
+template <int D, int NR>
 struct K8tSmem {
     static constexpr int STAGES = k8t_stages<D>;
-    static constexpr int P = 0;                                                    // two buffers of the weights' terms
-    static constexpr int Q = 2 * K8T_PTERMS * K8T_P_BYTES;
-    static constexpr int KV = Q + K8T_QTERMS * K8T_ROWS * D;                       // stages: K tile, V tile
+    static constexpr int S_COLS = 2 * NR < 16 ? 16 : 2 * NR;                       // scores' columns: term, head
+    static constexpr int O_COLS = 4 * NR < 16 ? 16 : 4 * NR;                       // outputs' columns: term, head
+    static constexpr int P_BYTES = O_COLS * K8T_KEYS;                              // [term, head][key], 128-byte swizzle
+    static constexpr int P = 0;                                                    // two of them
+    static constexpr int Q = 2 * P_BYTES;                                          // [term, head][d]
+    static constexpr int KV = Q + (S_COLS * D < 1024 ? 1024 : S_COLS * D);         // stages: K tile, V tile
     static constexpr int STAGE = 2 * K8T_KEYS * D;
     static constexpr int BARS = KV + STAGES * STAGE;
     static constexpr int MISC = BARS + (2 * STAGES + 6) * 8 + 16;
-    static constexpr int BYTES = MISC + (16 * 4 + 16 * 4 + 4 * 16 * 4);            // row factors, rescales, warps' maxima or sums
-    // the weights' operand is read as 128 rows: what lies behind its 16 has to be this CTA's
-    static_assert((2 * K8T_PTERMS - 1) * K8T_P_BYTES + 128 * K8T_KEYS <= BARS, "rows behind the weights' operand");
+    static constexpr int BYTES = MISC + (16 * 4 + 4 * 16 * 4);                     // row factors, warps' maxima or sums
     static_assert(Q % 1024 == 0 && KV % 1024 == 0, "swizzled tiles");
 };
 
@@ -133,7 +140,7 @@ struct K8tSmem {
 template <int D, int NR>
 __global__ void __launch_bounds__(K8T_THREADS)
 attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* out, const __grid_constant__ CUtensorMap map, const K8Args a) {
-    using L = K8tSmem<D>;
+    using L = K8tSmem<D, NR>;
     constexpr int STAGES = L::STAGES;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     pdl_launch_dependents();
@@ -148,9 +155,8 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
     auto pv_full = [&](int b) { return bars + (uint32_t)(2 * STAGES + 4 + b) * 8; };
     const uint32_t tmem_slot = bars + (2 * STAGES + 6) * 8;
     float* row_factor = reinterpret_cast<float*>(smem_raw + L::MISC);             // [16]
-    float* rescale = row_factor + 16;                                             // [16]
-    float* by_warp = rescale + 16;                                                // [4][16]
-    constexpr uint32_t COLS = D == 64 ? 128 : 256;                                // tensor memory: two of 16 columns for scores, then D
+    float* by_warp = row_factor + 16;                                             // [4][16]
+    constexpr uint32_t COLS = 128;                                                // tensor memory: two of up to 32 columns for scores, up to 64 for outputs
 
     if (tid == 0) {
         for (int i = 0; i < STAGES; ++i) {
@@ -223,9 +229,11 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
                     t2[h] |= (uint32_t)to_e4m3x2(u - back.x, v - back.y) << (16 * k);
                 }
             }
-            unsigned char* at = smem_raw + L::Q + swizzled<D>(r, (c0 + e) >> 4) + ((c0 + e) & 8);
-            *reinterpret_cast<uint2*>(at) = make_uint2(t1[0], t1[1]);
-            *reinterpret_cast<uint2*>(at + K8T_ROWS * D) = make_uint2(t2[0], t2[1]);
+            if (r < NR) {
+                unsigned char* at = smem_raw + L::Q + ((c0 + e) & 8);
+                *reinterpret_cast<uint2*>(at + swizzled<D>(r, (c0 + e) >> 4)) = make_uint2(t1[0], t1[1]);
+                *reinterpret_cast<uint2*>(at + swizzled<D>(NR + r, (c0 + e) >> 4)) = make_uint2(t2[0], t2[1]);
+            }
         }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -233,7 +241,7 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + (tmem_slot - base));
-    const uint32_t tmem_o = tmem + 32;
+    const uint32_t tmem_o = tmem + 64;
 
     if (warp == 4) {
         // ---- K and V: lane i brings positions [i per, (i + 1) per) of a tile, if any of them may be read ----
@@ -258,7 +266,8 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
         }
     } else if (warp == 5) {
         // ---- the products ----
-        constexpr uint32_t id_s = idesc8(K8T_ROWS, false), id_o = idesc8(D, true);
+        constexpr uint32_t id_s = idesc8(K8T_KEYS, L::S_COLS, false), id_o = idesc8(D, L::O_COLS, true);
+        const uint64_t qd = desc8<D>(base + L::Q);
         auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, k8_wait(bar, parity)) != 0; };
         bool ok = true;
         auto scores = [&](int j) {
@@ -269,11 +278,7 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
             const uint64_t kd = desc8<D>(base + L::KV + (uint32_t)s * L::STAGE);
             if (elect_lane()) {
 #pragma unroll
-                for (int t = 0; t < K8T_QTERMS; ++t) {
-                    const uint64_t qd = desc8<D>(base + L::Q + t * K8T_ROWS * D);
-#pragma unroll
-                    for (int k = 0; k < D / 32; ++k) umma_f8(tmem + (uint32_t)(j & 1) * 16, kd + 2 * k, qd + 2 * k, id_s, t + k > 0 ? 1u : 0u);
-                }
+                for (int k = 0; k < D / 32; ++k) umma_f8(tmem + (uint32_t)(j & 1) * 32, kd + 2 * k, qd + 2 * k, id_s, k > 0 ? 1u : 0u);
                 umma_commit(s_full(j & 1));
             }
             __syncwarp();
@@ -288,14 +293,11 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint64_t vd = desc8<D>(base + L::KV + (uint32_t)s * L::STAGE + K8T_KEYS * D);
+            const uint64_t pd = desc8<128>(base + L::P + b * L::P_BYTES);
             if (elect_lane()) {
 #pragma unroll
-                for (int t = 0; t < K8T_PTERMS; ++t) {
-                    const uint64_t pd = desc8<128>(base + L::P + (b * K8T_PTERMS + t) * K8T_P_BYTES);
-#pragma unroll
-                    for (int k = 0; k < K8T_KEYS / 32; ++k)
-                        umma_f8(tmem_o, pd + 2 * k, vd + (uint64_t)(k * 32 * D / 16), id_o, j + t + k > 0 ? 1u : 0u);
-                }
+                for (int k = 0; k < K8T_KEYS / 32; ++k)
+                    umma_f8(tmem_o, vd + (uint64_t)(k * 32 * D / 16), pd + 2 * k, id_o, j + k > 0 ? 1u : 0u);
                 umma_commit(pv_full(b));
                 umma_commit(kv_empty(s));
             }
@@ -339,7 +341,13 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
             ok = __all_sync(0xffffffffu, ok);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float x[NR];
-            tmem_ld_n<NR>(tmem + lanes + (uint32_t)b * 16, x);
+            {
+                constexpr int N = 2 * NR < 8 ? 8 : 2 * NR;
+                float sum[N];
+                tmem_ld_n<N>(tmem + lanes + (uint32_t)b * 32, sum);
+#pragma unroll
+                for (int r = 0; r < NR; ++r) x[r] = sum[r] + sum[NR + r];
+            }
             bool above = false;
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
@@ -353,35 +361,31 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
                     if (lane == 0) by_warp[warp * 16 + r] = top;
                 }
                 sync_128();
+                float f[NR];
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
                     const float top = fmaxf(fmaxf(by_warp[r], by_warp[16 + r]), fmaxf(by_warp[32 + r], by_warp[48 + r]));
-                    const float m_new = fmaxf(m[r], top), f = m_new == -INFINITY ? 1.f : k8_exp2(m[r] - m_new);
+                    const float m_new = fmaxf(m[r], top);
+                    f[r] = m_new == -INFINITY ? 1.f : k8_exp2(m[r] - m_new);
                     m[r] = m_new;
-                    l[r] *= f;
-                    if (tid == 0) rescale[r] = f;
+                    l[r] *= f[r];
                 }
-                if (warp == 0 && it > 0) {
-                    // what the first 32 lanes of tensor memory have accumulated (no product is under way once the last tile's is done)
+                if (it > 0) {
+                    // what this warp's lanes have accumulated (no product is under way once the last tile's is done)
                     if (ok) ok = k8_wait(pv_full(b ^ 1), (uint32_t)(((it - 1) >> 1) & 1));
                     ok = __all_sync(0xffffffffu, ok);
-                    __syncwarp();
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const float f = (lane & 15) < NR ? rescale[lane & 15] : 0.f;
+                    float v[L::O_COLS];
+                    tmem_ld_n<L::O_COLS>(tmem_o + lanes, v);
 #pragma unroll
-                    for (int col = 0; col < D; col += 16) {
-                        float v[16];
-                        tmem_ld16(tmem_o + (uint32_t)col, v);
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) v[e] = (lane & 15) < NR ? v[e] * f : 0.f;
-                        tmem_st16(tmem_o + (uint32_t)col, v);
-                    }
+                    for (int i = 0; i < K8T_PTERMS * NR; ++i) v[i] *= f[i % NR];
+                    tmem_st_n<L::O_COLS>(tmem_o + lanes, v);
                 }
                 sync_128();                              // (the warps' maxima are read; they are written again at the next raise)
             }
             // the terms of tile it - 2 have been read
             if (ok && it >= 2) ok = k8_wait(pv_full(b), (uint32_t)((turn - 1) & 1));
-            unsigned char* p = smem_raw + L::P + b * (K8T_PTERMS * K8T_P_BYTES);
+            unsigned char* p = smem_raw + L::P + b * L::P_BYTES + (tid & 15);
 #pragma unroll
             for (int r = 0; r < NR; r += 2) {
                 float w[2];
@@ -390,17 +394,18 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
                     w[h] = k8_exp2(x[r + h] + (m[r + h] == -INFINITY ? 0.f : K8T_LIFT - m[r + h]));
                     l[r + h] = fmaf(w[h], inv_v, l[r + h]);
                 }
-                const uint32_t at0 = swizzled<128>(r, tid >> 4) + (tid & 15), at1 = swizzled<128>(r + 1, tid >> 4) + (tid & 15);
 #pragma unroll
-                for (int t = 0; t < 2 * K8T_PTERMS; ++t) {
+                for (int t = 0; t < K8T_PTERMS; ++t) {
                     const uint16_t two = to_e4m3x2(w[0], w[1]);
-                    unsigned char* term = p + (t % K8T_PTERMS) * K8T_P_BYTES + (t / K8T_PTERMS) * (K8T_ROWS * K8T_KEYS);
-                    term[at0] = (unsigned char)two;
-                    term[at1] = (unsigned char)(two >> 8);
+                    p[swizzled<128>(t * NR + r, tid >> 4)] = (unsigned char)two;
+                    p[swizzled<128>(t * NR + r + 1, tid >> 4)] = (unsigned char)(two >> 8);
                     const float2 back = half2_floats(e4m3x2_to_half2(two));
-                    const float up = t == K8T_PTERMS - 1 ? K8T_FINE : 1.f;
-                    w[0] = (w[0] - back.x) * up;
-                    w[1] = (w[1] - back.y) * up;
+                    w[0] -= back.x;
+                    w[1] -= back.y;
+                    if (t == 1) {
+                        w[0] *= K8T_FINE;
+                        w[1] *= K8T_FINE;
+                    }
                 }
             }
             if (!seen) {
@@ -414,57 +419,38 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full(b));
         }
-        // ---- the sums over keys, then a row a lane of the first warp ----
+        // ---- the sums over keys, then a column of the head a lane (D = 64: the products leave 16 in each warp's lanes) ----
         sync_128();
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             const float sum = warp_sum(l[r]);
             if (lane == 0) by_warp[warp * 16 + r] = sum;
-            if (tid == 0) rescale[r] = m[r];
         }
+        if (ok && n_tiles > 0) ok = k8_wait(pv_full((n_tiles - 1) & 1), (uint32_t)(((n_tiles - 1) >> 1) & 1));
+        ok = __all_sync(0xffffffffu, ok);
         sync_128();
-        if (warp == 0) {
-            if (ok && n_tiles > 0) ok = k8_wait(pv_full((n_tiles - 1) & 1), (uint32_t)(((n_tiles - 1) >> 1) & 1));
-            ok = __all_sync(0xffffffffu, ok);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const int r = lane < NR ? lane : 0;
-            const bool mine = lane < G && tok >= 0;
-            const float m_r = rescale[r];
-            float l_r = by_warp[r] + by_warp[16 + r] + by_warp[32 + r] + by_warp[48 + r];
-            const int head = kvh * G + lane;
-            float inv = 1.f, gate = 1.f;
-            float* part = nullptr;
-            if (a.nsplit == 1) {
-                if (a.sink && m_r > -INFINITY) l_r += k8_exp2(K8T_LIFT - m_r);
-                inv = l_r == 0.f ? 0.f : 1.f / l_r;
-                if (mine) gate = k8_gate<__nv_bfloat16>(a, tok, head);
-            } else if (mine) {
-                part = a.scratch + ((((size_t)item * a.Hkv + kvh) * a.nsplit + split) * a.rows_most + lane) * (D + 4);
-                *reinterpret_cast<float2*>(part + D) = make_float2(m_r, l_r);
-            }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        float v[L::O_COLS];
 #pragma unroll
-            for (int col = 0; col < D; col += 16) {
-                float v[16];
-                if (n_tiles > 0) tmem_ld16(tmem_o + (uint32_t)col, v);
+        for (int i = 0; i < L::O_COLS; ++i) v[i] = 0.f;
+        if (n_tiles > 0) tmem_ld_n<L::O_COLS>(tmem_o + lanes, v);
+        constexpr int PER = D / 4;
+        const int d = warp * PER + lane;
+        if (tok >= 0 && lane < PER) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float fine = __shfl_down_sync(0xffffffffu, v[e], 16);
-                    v[e] = n_tiles > 0 ? fmaf(fine, 1.f / K8T_FINE, v[e]) * inv : 0.f;
-                }
-                if (!mine) continue;
-                if (part != nullptr) {
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(part + col + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            for (int r = 0; r < NR; ++r) {
+                if (r >= G) continue;
+                float o = fmaf(v[2 * NR + r] + v[3 * NR + r], 1.f / K8T_FINE, v[r] + v[NR + r]);
+                float l_r = (by_warp[r] + by_warp[16 + r]) + (by_warp[32 + r] + by_warp[48 + r]);
+                const int head = kvh * G + r;
+                if (a.nsplit == 1) {
+                    if (a.sink && m[r] > -INFINITY) l_r += k8_exp2(K8T_LIFT - m[r]);
+                    o = l_r == 0.f ? 0.f : o / l_r;
+                    out[((size_t)tok * a.H + head) * D + d] = __float2bfloat16_rn(k8_apply<__nv_bfloat16>(o, a, k8_gate<__nv_bfloat16>(a, tok, head)));
                 } else {
-                    uint32_t packed[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const __nv_bfloat162 y = __floats2bfloat162_rn(k8_apply<__nv_bfloat16>(v[2 * e], a, gate), k8_apply<__nv_bfloat16>(v[2 * e + 1], a, gate));
-                        packed[e] = *reinterpret_cast<const uint32_t*>(&y);
-                    }
-                    uint4* dst = reinterpret_cast<uint4*>(out + ((size_t)tok * a.H + head) * D + col);
-                    dst[0] = make_uint4(packed[0], packed[1], packed[2], packed[3]);
-                    dst[1] = make_uint4(packed[4], packed[5], packed[6], packed[7]);
+                    float* part = a.scratch + ((((size_t)item * a.Hkv + kvh) * a.nsplit + split) * a.rows_most + r) * (D + 4);
+                    part[d] = o;
+                    if (d == 0) *reinterpret_cast<float2*>(part + D) = make_float2(m[r], l_r);
                 }
             }
         }
@@ -492,7 +478,7 @@ bool k8t_map(CUtensorMap* map, const void* pool, int D, int P) {
 
 template <int D, int NR>
 cudaError_t k8t_launch(const void* q, const float* scales, void* out, const CUtensorMap& map, const K8Args& a, cudaStream_t stream) {
-    constexpr int smem = K8tSmem<D>::BYTES;
+    constexpr int smem = K8tSmem<D, NR>::BYTES;
     cudaError_t e = cudaFuncSetAttribute(attn_kv8_tc_kernel<D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     return tk_launch(attn_kv8_tc_kernel<D, NR>, dim3((unsigned)(a.items * a.Hkv * a.nsplit)), dim3(K8T_THREADS), smem, stream, (const __nv_bfloat16*)q,
