@@ -444,14 +444,32 @@ TK_API int tk_attn_kv8_supported(int H, int Hkv, int D) {
 // Tokens of one sequence a tile of tk_attn_kv8 has.
 TK_API int tk_attn_kv8_tokens(int H, int Hkv) { return K8_ROWS / (H / Hkv); }
 
-// Ways to share the keys of each of `items` rows' tiles out over CTAs, when no sequence holds more than `longest` positions.
-TK_API int tk_attn_kv8_splits(int items, int Hkv, int longest, int sm_count) {
+// Ways to share the keys of each of `items` tiles out over CTAs, when no sequence holds more than `longest` positions and a query sees at most `reach` of them. tc:
+// single tokens through the tcgen05 kernel: as many as keep every CTA resident (four an SM for heads of 64 with up to four query heads a KV head, else two: one
+// CTA more and the launch runs in two waves), in clusters of at most eight with two tiles of 128 keys each, or of 16 with four (us by shares, 8 KV heads of 64:
+// a token behind 2,048 positions 14.9 unshared, 8.7 by 4, 7.6 by 8, 8.5 by 16; behind 30,000 136, 40, 24.7, 20.8; 8 tokens behind 32,000 49.0 by 6, 45.7 by 8, 61.7
+// by 10; 16 behind 4,000 15.3 by 4, 20.3 by 5; 64 behind up to 3,000 33.1 unshared, 38.9 by 2).
+// The mma.sync kernel's shares meet in scratch memory: enough to put four CTAs on every SM, of 256 keys at least.
+TK_API int tk_attn_kv8_splits(int items, int H, int Hkv, int D, int longest, int reach, int sm_count, int tc) {
     const int64_t ctas = (int64_t)items * Hkv;
     if (ctas <= 0) return 1;
-    const int64_t fill = (4 * (int64_t)sm_count + ctas - 1) / ctas, keys = (longest + 255) / 256;
-    const int64_t n = fill < keys ? fill : keys;
-    return (int)(n < 1 ? 1 : n > 128 ? 128 : n);
+    const int64_t keys = longest < reach ? longest : reach;
+    if (!tc) {
+        const int64_t fill = (4 * (int64_t)sm_count + ctas - 1) / ctas, by_keys = (keys + 255) / 256;
+        const int64_t n = fill < by_keys ? fill : by_keys;
+        return (int)(n < 1 ? 1 : n > 128 ? 128 : n);
+    }
+    const int64_t fit = (int64_t)sm_count * (D == 64 && H / Hkv <= 4 ? 4 : 2) / ctas, tiles = (keys + 127) / 128 + (reach < longest ? 1 : 0);
+    if (fit >= 16 && tiles >= 64) return 16;
+    int64_t n = (tiles + 1) / 2;
+    if (n < 4) n = tiles < 4 ? tiles : 4;
+    if (n > 8) n = 8;
+    if (n > fit) n = fit;
+    return (int)(n < 1 ? 1 : n);
 }
+
+// Whether single tokens of this shape take the tcgen05 kernel: 16-bit queries, pages that are a power of two and 16 or more positions.
+TK_API int tk_attn_kv8_single_tc(int P, int dtype) { return dtype == TK_BF16 && P >= 16 && (P & (P - 1)) == 0; }
 
 int tk_attn_kv8_tc(const void* q, const void* pool, const float* scales, void* out, const void* args, int D, cudaStream_t stream);
 int tk_attn_kv8_tc_status();
@@ -474,7 +492,7 @@ TK_API int tk_attn_kv8(const void* q, const void* pool, const float* scales, voi
                        cudaStream_t stream) {
     TK_CHECK_ARG(tk_attn_kv8_supported(H, Hkv, D), "attn_kv8: shape H=%d Hkv=%d D=%d is not taken (heads of 64 or 128, up to %d a KV head)", H,
                  Hkv, D, K8_ROWS);
-    TK_CHECK_ARG(items >= 0 && P > 0 && nsplit >= 1 && (nsplit == 1 || scratch != nullptr), "attn_kv8: bad sizes");
+    TK_CHECK_ARG(items >= 0 && P > 0 && nsplit >= 1 && (nsplit == 1 || scratch != nullptr || (item_ntok == nullptr && tk_attn_kv8_single_tc(P, dtype))), "attn_kv8: bad sizes");
     TK_CHECK_ARG(item_ntok == nullptr || item_tok0 != nullptr, "attn_kv8: tiles have first tokens");
     TK_CHECK_ARG((int64_t)items * Hkv * nsplit < 0x7fffffff, "attn_kv8: %d splits of %d items", nsplit, items);
     TK_CHECK_ARG(scale > 0.f, "attn_kv8: the scores' factor is positive");
@@ -487,8 +505,10 @@ TK_API int tk_attn_kv8(const void* q, const void* pool, const float* scales, voi
     const int G = H / Hkv;
     K8Args a{positions, tok_seq, block_table, item_tok0, item_ntok, gate, scratch, ldg, bt_stride, items, H, Hkv, P, shift, window, nsplit, sink,
              item_ntok != nullptr ? (K8_ROWS / G) * G : G, scale};
-    // single tokens of 16-bit models whose pages a tensor map can follow
-    if (dtype == TK_BF16 && item_ntok == nullptr && shift >= 4) return tk_attn_kv8_tc(q, pool, scales, out, &a, D, stream);
+    if (item_ntok == nullptr && tk_attn_kv8_single_tc(P, dtype)) {
+        TK_CHECK_ARG(nsplit <= 16, "attn_kv8: %d shares of a token's keys (at most 16)", nsplit);
+        return tk_attn_kv8_tc(q, pool, scales, out, &a, D, stream);
+    }
     const cudaError_t e = dtype == TK_F32 ? k8_dispatch<float>(q, pool, scales, out, a, D, stream)
                                           : k8_dispatch<__nv_bfloat16>(q, pool, scales, out, a, D, stream);
     if (e != cudaSuccess) {

@@ -8,31 +8,35 @@
 // division by a power of two that brings its row's largest to [128, 256)) is two terms, exactly for elements down to 2^-12 of the row's
 // largest and to 2^-18 of that below. A weight is four: two that leave 2^-8 of it or 2^-10 (e4m3's smallest steps), and two of what they leave times
 // 2^8. The weights' reference maximum follows lazily (raised when a row exceeds it by 2^2) and weights are lifted by 2^6 (at most 256, of 448): a
-// weight is off by at most 2^-16 of itself or 2^-24 of the row's largest. (Two terms alone lose the many small weights beside a large one: 30,000
+// weight (rounded to float16 first, so that the terms are packed arithmetic) is off by at most 2^-11 of itself or 2^-24 of the row's largest. (Two terms alone lose the many small weights beside a large one: 30,000
 // keys that share half of a row's weight with one that has the other half would be off by a tenth.) A value block's scale is in the
 // exponent, as in attention_kv8.cu. Columns cost nothing here: a product's time is that of reading its 128 x 32 or D x 32 bytes of the first operand
 // from shared memory. (With the heads as the M side of the second product, 32 rows of 128, and the terms one after the other, the products
 // alone took 575 cycles a tile of 128 keys, and 8 tokens behind 32,000 positions 71 us.)
 //
-// A CTA takes the query heads of one KV head of one token and a share of its keys, in tiles of 128:
-//   warp 4      brings K and V by TMA, a page (or 128 positions of one) a load, two or three tiles ahead
-//   warp 5      issues the products
+// A CTA takes the query heads of one KV head of one token and a share of its keys, in tiles of 128 (up to 16 CTAs, a cluster, share them and join
+// their shares through each other's shared memory):
+//   warps 4, 5  bring K and V by TMA, a page (or 128 positions of one) a load, up to three tiles ahead
+//   warp 6      issues the products
 //   warps 0-3   thread = key: masks, reference maximum (one vote of the four warps a tile), weights, their terms into shared memory
 //               ([term and head][key], the second product's other operand); positions that are not to be seen have their value rows zeroed there
 //
 // Masking and sums are those of attention_kv8.cu; every wait is bounded (about a second), the kernel then frees its tensor memory and
 // returns, and tk_attn_kv8_status() says so.
+#include <cooperative_groups.h>
 #include <math.h>
 
-#include "kv8.cuh"
 #include "kv8_attn.cuh"
 #include "tcgen05.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace {
 
-constexpr int K8T_KEYS = 128, K8T_ROWS = 16;
-constexpr int K8T_THREADS = 192;
-constexpr int K8T_QTERMS = 2, K8T_PTERMS = 4;
+constexpr int K8T_KEYS = 128;
+constexpr int K8T_COPIERS = 2;                             // warps that bring keys, and values
+constexpr int K8T_MMA_WARP = 4 + K8T_COPIERS, K8T_THREADS = (K8T_MMA_WARP + 1) * 32;
+constexpr int K8T_PTERMS = 4;
 constexpr float K8T_LAZY = 2.0f, K8T_LIFT = 6.0f, K8T_FINE = 256.0f;
 
 // K-major or MN-major operand whose rows are D = 64 (64-byte swizzle) or 128 bytes (128-byte swizzle), groups of eight rows one after the other
@@ -116,9 +120,9 @@ __device__ __forceinline__ bool any_of_128(bool mine) {
 }
 __device__ __forceinline__ void sync_128() { asm volatile("bar.sync 2, 128;" ::: "memory"); }
 
-// tiles of keys and values in shared memory: as many as leave room for three CTAs an SM (D = 64), or two
+// tiles of keys and values in shared memory (they leave room for three CTAs an SM, heads of 128 for two)
 template <int D>
-constexpr int k8t_stages = D == 64 ? 3 : 2;
+constexpr int k8t_stages = 3;
 
 template <int D, int NR>
 struct K8tSmem {
@@ -131,14 +135,18 @@ struct K8tSmem {
     static constexpr int KV = Q + (S_COLS * D < 1024 ? 1024 : S_COLS * D);         // stages: K tile, V tile
     static constexpr int STAGE = 2 * K8T_KEYS * D;
     static constexpr int BARS = KV + STAGES * STAGE;
-    static constexpr int MISC = BARS + (2 * STAGES + 6) * 8 + 16;
+    static constexpr int SCALES = BARS + (2 * STAGES + 6) * 8 + 16;                // of a tile's eight groups of 16 keys: (key's, value's)
+    static constexpr int MISC = SCALES + STAGES * 8 * 8;
     static constexpr int BYTES = MISC + (16 * 4 + 4 * 16 * 4);                     // row factors, warps' maxima or sums
+    static_assert(SCALES % 8 == 0 && MISC % 8 == 0, "pairs");
+    // a share of the keys, for the CTAs that join theirs: [head][d] and the heads' maxima and sums, where the first tiles were
+    static_assert(NR * (D + 2) * 4 <= STAGES * STAGE, "a share");
     static_assert(Q % 1024 == 0 && KV % 1024 == 0, "swizzled tiles");
 };
 
 // D: head size; NR: query heads a KV head has, rounded up to 2, 4, 8 or 16
 template <int D, int NR>
-__global__ void __launch_bounds__(K8T_THREADS)
+__global__ void __launch_bounds__(K8T_THREADS, D == 64 && NR <= 4 ? 4 : 2)
 attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* out, const __grid_constant__ CUtensorMap map, const K8Args a) {
     using L = K8tSmem<D, NR>;
     constexpr int STAGES = L::STAGES;
@@ -156,11 +164,13 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
     const uint32_t tmem_slot = bars + (2 * STAGES + 6) * 8;
     float* row_factor = reinterpret_cast<float*>(smem_raw + L::MISC);             // [16]
     float* by_warp = row_factor + 16;                                             // [4][16]
+    float* share = reinterpret_cast<float*>(smem_raw + L::KV);                    // [head][d]
+    float2* share_ml = reinterpret_cast<float2*>(share + NR * D);
     constexpr uint32_t COLS = 128;                                                // tensor memory: two of up to 32 columns for scores, up to 64 for outputs
 
     if (tid == 0) {
         for (int i = 0; i < STAGES; ++i) {
-            mbar_init(kv_full(i), 1);
+            mbar_init(kv_full(i), K8T_COPIERS);
             mbar_init(kv_empty(i), 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -171,7 +181,7 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 5) {
+    if (warp == K8T_MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -243,28 +253,48 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + (tmem_slot - base));
     const uint32_t tmem_o = tmem + 64;
 
-    if (warp == 4) {
-        // ---- K and V: lane i brings positions [i per, (i + 1) per) of a tile, if any of them may be read ----
-        const int per_log = min(a.p_shift, 7), per = 1 << per_log;
+    if (warp >= 4 && warp < K8T_MMA_WARP) {
+        // ---- K and V: lane i knows the page and the scales of 16 positions of one of four tiles, and brings the page (or 128 positions of it)
+        // if they are its first of the tile: keys one warp, values the other. (A warp's loads go out one after the other, 65 to 100 cycles
+        // each however they are issued: one warp for a tile's 16 set the pace at 1,450 cycles a tile.) The pages of four tiles are asked for
+        // eight tiles ahead, their scales four: no trip is waited for. ----
+        const int which = warp - 4, per = 1 << min(a.p_shift, 7);
+        const int group = lane & 7, at_row = (group * 16) & (per - 1);        // (of a page, as far as a tile reaches)
         bool ok = true;
+        auto page_of = [&](int four) {
+            const int it = four * 4 + (lane >> 3), j = (t_begin + it) * K8T_KEYS + group * 16 - at_row;
+            return it < n_tiles && j <= pos && j + per > lo ? TK_PAGE(TK_K_KV8_ATTN, bt[j >> a.p_shift]) : -1;
+        };
+        auto scales_of = [&](int pg) {
+            const float* from = scales + (size_t)max(pg, 0) * (2 * a.Hkv) + kvh;
+            return pg >= 0 ? make_float2(from[0], from[a.Hkv]) : make_float2(1.f, 1.f);
+        };
+        int page = -1, page_next = page_of(0), page_after = page_of(1);
+        float2 scale = make_float2(1.f, 1.f), scale_next = scales_of(page_next);
+        float2* sc = reinterpret_cast<float2*>(smem_raw + L::SCALES);
         for (int it = 0; it < n_tiles; ++it) {
-            const int s = it % STAGES, j = (t_begin + it) * K8T_KEYS + lane * per;
-            const bool mine = lane < (K8T_KEYS >> per_log) && j <= pos && j + per > lo;
-            int page = 0;
-            if (mine) page = TK_PAGE(TK_K_KV8_ATTN, bt[j >> a.p_shift]);
+            const int s = it % STAGES;
+            if ((it & 3) == 0) {
+                page = page_next;
+                scale = scale_next;
+                page_next = page_after;
+                scale_next = scales_of(page_next);
+                page_after = page_of(it / 4 + 2);
+            }
             if (it >= STAGES) ok = k8_wait(kv_empty(s), (uint32_t)((it / STAGES - 1) & 1));
             if (!__all_sync(0xffffffffu, ok)) break;
+            const bool ours = (lane >> 3) == (it & 3), mine = ours && page >= 0 && at_row == 0;
             const int loads = __popc(__ballot_sync(0xffffffffu, mine));
-            if (lane == 0) mbar_expect_tx(kv_full(s), (uint32_t)(loads * 2 * per * D));
-            __syncwarp();
             if (mine) {
-                const int row = ((page * 2) * a.Hkv + kvh) * P + (j & (P - 1));
-                const uint32_t at = base + L::KV + (uint32_t)s * L::STAGE + (uint32_t)(lane * per * D);
-                tma_load_2d(at, &map, 0, row, kv_full(s));
-                tma_load_2d(at + K8T_KEYS * D, &map, 0, row + a.Hkv * P, kv_full(s));
+                const int row = ((page * 2 + which) * a.Hkv + kvh) * P + (((t_begin + it) * K8T_KEYS + group * 16) & (P - 1));
+                tma_load_2d(base + L::KV + (uint32_t)s * L::STAGE + (uint32_t)((which * K8T_KEYS + group * 16) * D), &map, 0, row, kv_full(s));
             }
+            if (which == 0 && ours) sc[s * 8 + group] = scale;
+            __syncwarp();
+            // (the phase ends with this arrival and the bytes, whichever come last)
+            if (lane == 0) mbar_expect_tx(kv_full(s), (uint32_t)(loads * per * D));
         }
-    } else if (warp == 5) {
+    } else if (warp == K8T_MMA_WARP) {
         // ---- the products ----
         constexpr uint32_t id_s = idesc8(K8T_KEYS, L::S_COLS, false), id_o = idesc8(D, L::O_COLS, true);
         const uint64_t qd = desc8<D>(base + L::Q);
@@ -314,31 +344,15 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
         }
         const uint32_t lanes = (uint32_t)(warp * 32) << 16;
         bool ok = true;
-        // a key's page is looked up two tiles ahead of its use, its scales one
-        auto page_of = [&](int it) {
-            const int j = (t_begin + it) * K8T_KEYS + tid;
-            return it < n_tiles && j >= lo && j <= pos ? TK_PAGE(TK_K_KV8_ATTN, bt[j >> a.p_shift]) : -1;
-        };
-        int page = page_of(0);
-        float ks = 1.f, vs = 1.f;
-        auto scales_of = [&](int pg) {
-            const float* sc = scales + (size_t)max(pg, 0) * (2 * a.Hkv) + kvh;
-            ks = pg >= 0 ? sc[0] : 1.f;
-            vs = pg >= 0 ? sc[a.Hkv] : 1.f;
-        };
-        scales_of(page);
-        page = page_of(1);
         for (int it = 0; it < n_tiles; ++it) {
             const int b = it & 1, turn = it >> 1, j = (t_begin + it) * K8T_KEYS + tid;
             const bool seen = j >= lo && j <= pos;
-            const float k_now = ks;
-            const int bits = __float_as_int(vs);
-            const float ev = __int_as_float(0x4b000000 | (bits >> 23)) - 8388735.0f, inv_v = __int_as_float((254 << 23) - bits);
-            scales_of(page);
-            page = page_of(it + 2);
             // (after a failed wait the loop runs to its end without waiting: every thread meets every barrier)
-            if (ok) ok = k8_wait(s_full(b), (uint32_t)(turn & 1));
+            if (ok) ok = k8_wait(s_full(b), (uint32_t)(turn & 1)) && k8_wait(kv_full(it % STAGES), (uint32_t)((it / STAGES) & 1));
             ok = __all_sync(0xffffffffu, ok);
+            const float2 sc = reinterpret_cast<const float2*>(smem_raw + L::SCALES)[(it % STAGES) * 8 + (tid >> 4)];
+            const int bits = __float_as_int(sc.y);
+            const float ev = __int_as_float(0x4b000000 | (bits >> 23)) - 8388735.0f, inv_v = __int_as_float((254 << 23) - bits);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float x[NR];
             {
@@ -351,7 +365,7 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
             bool above = false;
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-                x[r] = seen ? fmaf(x[r], k_now * c[r], ev) : -INFINITY;
+                x[r] = seen ? fmaf(x[r], sc.x * c[r], ev) : -INFINITY;
                 above = above || x[r] > m[r] + K8T_LAZY;
             }
             if (any_of_128(above)) {
@@ -394,18 +408,16 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
                     w[h] = k8_exp2(x[r + h] + (m[r + h] == -INFINITY ? 0.f : K8T_LIFT - m[r + h]));
                     l[r + h] = fmaf(w[h], inv_v, l[r + h]);
                 }
+                __half2 left = __floats2half2_rn(w[0], w[1]);        // (what a term leaves of a float16 is one)
 #pragma unroll
                 for (int t = 0; t < K8T_PTERMS; ++t) {
-                    const uint16_t two = to_e4m3x2(w[0], w[1]);
+                    uint16_t two;
+                    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(two) : "r"(*reinterpret_cast<const uint32_t*>(&left)));
                     p[swizzled<128>(t * NR + r, tid >> 4)] = (unsigned char)two;
                     p[swizzled<128>(t * NR + r + 1, tid >> 4)] = (unsigned char)(two >> 8);
-                    const float2 back = half2_floats(e4m3x2_to_half2(two));
-                    w[0] -= back.x;
-                    w[1] -= back.y;
-                    if (t == 1) {
-                        w[0] *= K8T_FINE;
-                        w[1] *= K8T_FINE;
-                    }
+                    const uint32_t back = e4m3x2_to_half2(two);
+                    left = __hsub2(left, *reinterpret_cast<const __half2*>(&back));
+                    if (t == 1) left = __hmul2(left, __float2half2_rn(K8T_FINE));
                 }
             }
             if (!seen) {
@@ -448,16 +460,38 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
                     o = l_r == 0.f ? 0.f : o / l_r;
                     out[((size_t)tok * a.H + head) * D + d] = __float2bfloat16_rn(k8_apply<__nv_bfloat16>(o, a, k8_gate<__nv_bfloat16>(a, tok, head)));
                 } else {
-                    float* part = a.scratch + ((((size_t)item * a.Hkv + kvh) * a.nsplit + split) * a.rows_most + r) * (D + 4);
-                    part[d] = o;
-                    if (d == 0) *reinterpret_cast<float2*>(part + D) = make_float2(m[r], l_r);
+                    share[r * D + d] = o;
+                    if (d == 0) share_ml[r] = make_float2(m[r], l_r);
                 }
             }
         }
     }
+    if (a.nsplit > 1) {
+        // each CTA forms an equal part of the outputs from all shares, through the cluster's shared memory
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        if (tok >= 0) {
+            for (int i = split * K8T_THREADS + tid; i < G * D; i += a.nsplit * K8T_THREADS) {
+                const int r = i / D, d = i % D, head = kvh * G + r;
+                float m_all = -INFINITY, l_all = 0.f, o = 0.f;
+                for (int sp = 0; sp < a.nsplit; ++sp) m_all = fmaxf(m_all, cluster.map_shared_rank(share_ml, sp)[r].x);
+#pragma unroll 4
+                for (int sp = 0; sp < a.nsplit; ++sp) {
+                    const float2 ml = cluster.map_shared_rank(share_ml, sp)[r];
+                    const float f = k8_factor(ml.x, ml.y, m_all);
+                    l_all = fmaf(ml.y, f, l_all);
+                    o = fmaf(cluster.map_shared_rank(share, sp)[r * D + d], f, o);
+                }
+                if (a.sink && m_all > -INFINITY) l_all += k8_exp2(K8T_LIFT - m_all);
+                o = l_all == 0.f ? 0.f : o / l_all;
+                out[((size_t)tok * a.H + head) * D + d] = __float2bfloat16_rn(k8_apply<__nv_bfloat16>(o, a, k8_gate<__nv_bfloat16>(a, tok, head)));
+            }
+        }
+        cluster.sync();                                  // nobody leaves while its share is read
+    }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 5) {
+    if (warp == K8T_MMA_WARP) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS) : "memory");
     }
@@ -480,21 +514,37 @@ template <int D, int NR>
 cudaError_t k8t_launch(const void* q, const float* scales, void* out, const CUtensorMap& map, const K8Args& a, cudaStream_t stream) {
     constexpr int smem = K8tSmem<D, NR>::BYTES;
     cudaError_t e = cudaFuncSetAttribute(attn_kv8_tc_kernel<D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && a.nsplit > 8) e = cudaFuncSetAttribute(attn_kv8_tc_kernel<D, NR>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
-    return tk_launch(attn_kv8_tc_kernel<D, NR>, dim3((unsigned)(a.items * a.Hkv * a.nsplit)), dim3(K8T_THREADS), smem, stream, (const __nv_bfloat16*)q,
-                     scales, (__nv_bfloat16*)out, map, a);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.items * a.Hkv * a.nsplit));
+    cfg.blockDim = dim3(K8T_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (tk_pdl_enabled()) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (a.nsplit > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = (unsigned)a.nsplit;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    return cudaLaunchKernelEx(&cfg, attn_kv8_tc_kernel<D, NR>, (const __nv_bfloat16*)q, scales, (__nv_bfloat16*)out, map, a);
 }
 
 template <int D>
 cudaError_t k8t_rows(const void* q, const float* scales, void* out, const CUtensorMap& map, const K8Args& a, cudaStream_t stream) {
     const int G = a.H / a.Hkv;
-    cudaError_t e = G <= 2   ? k8t_launch<D, 2>(q, scales, out, map, a, stream)
-                    : G <= 4 ? k8t_launch<D, 4>(q, scales, out, map, a, stream)
-                    : G <= 8 ? k8t_launch<D, 8>(q, scales, out, map, a, stream)
-                             : k8t_launch<D, 16>(q, scales, out, map, a, stream);
-    if (e != cudaSuccess || a.nsplit == 1) return e;
-    const unsigned grid = (unsigned)(((int64_t)a.items * a.Hkv * a.rows_most + 3) / 4);
-    return tk_launch(attn_kv8_merge_kernel<__nv_bfloat16, D>, dim3(grid), dim3(128), 0, stream, (__nv_bfloat16*)out, a, K8T_LIFT);
+    return G <= 2   ? k8t_launch<D, 2>(q, scales, out, map, a, stream)
+           : G <= 4 ? k8t_launch<D, 4>(q, scales, out, map, a, stream)
+           : G <= 8 ? k8t_launch<D, 8>(q, scales, out, map, a, stream)
+                    : k8t_launch<D, 16>(q, scales, out, map, a, stream);
 }
 
 }  // namespace

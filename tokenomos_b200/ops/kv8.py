@@ -16,7 +16,7 @@ import torch
 
 from tokenomos_b200 import ops
 from tokenomos_b200.ops import _lib
-from tokenomos_b200.ops._lib import KernelError
+from tokenomos_b200.ops._lib import BF16, KernelError
 
 KV8_DTYPE = torch.float8_e4m3fn
 
@@ -112,10 +112,11 @@ def _sms(device: torch.device) -> int:
 
 def _attend(q, pool, scales, out, positions, tok_seq, block_table, tok0, ntok, items, rows, shape, window, scale, longest, gate, sink):
     T, H, Hkv, P, D, code = shape
-    reach = abs(int(window)) if window else longest
-    nsplit = _lib.call("tk_attn_kv8_splits", items, Hkv, max(1, min(int(longest), reach + rows)), _sms(q.device))
+    reach = abs(int(window)) + rows - 1 if window else longest
+    tc = ntok is None and code == BF16 and P >= 16 and not P & (P - 1)
+    nsplit = _lib.call("tk_attn_kv8_splits", items, H, Hkv, D, int(longest), reach, _sms(q.device), tc)
     scratch = None
-    if nsplit > 1:
+    if nsplit > 1 and not tc:
         scratch = torch.empty(items * Hkv * nsplit * rows * (H // Hkv) * (D + 4), dtype=torch.float32, device=q.device)
     _lib.call("tk_attn_kv8", q.data_ptr(), pool.data_ptr(), scales.data_ptr(), out.data_ptr(), positions.data_ptr(), tok_seq.data_ptr(),
               block_table.data_ptr(), block_table.stride(0), ops._ptr(tok0), ops._ptr(ntok), items, H, Hkv, D, P, int(window or 0),
