@@ -654,7 +654,9 @@ def test_entry_points_refuse_shapes_that_are_not_built():
     with pytest.raises(KernelError, match="positive"):
         _lib.call("tk_attn_kv8", 256, 256, 256, 256, 256, 256, 256, 1, None, None, 1, 4, 2, 64, 16, 0, 0.0, 1, None, None, 0, 0, 1, None)
     with pytest.raises(KernelError, match="bad sizes"):
-        _lib.call("tk_attn_kv8", 256, 256, 256, 256, 256, 256, 256, 1, None, None, 1, 4, 2, 64, 16, 0, 1.0, 4, None, None, 0, 0, 1, None)
+        _lib.call("tk_attn_kv8", 256, 256, 256, 256, 256, 256, 256, 1, None, None, 1, 4, 2, 64, 16, 0, 1.0, 4, None, None, 0, 0, 0, None)
+    with pytest.raises(KernelError, match="at most 16"):
+        _lib.call("tk_attn_kv8", 256, 256, 256, 256, 256, 256, 256, 1, None, None, 1, 4, 2, 64, 16, 0, 1.0, 17, None, None, 0, 0, 1, None)
 
 
 def test_tensors_of_the_host_are_refused():

@@ -85,15 +85,15 @@ class _Worker(threading.Thread):
 
 class LLM:
     def __init__(self, model: str, device: str = "cuda", arch=None, work: str | None = None,
-                 **engine_kw):
+                 cache: str | None = None, **engine_kw):
         """``model``: a folder with config.json and safetensors. ``arch``: what
         ``models.configure(folder, work=...)`` returned, when the caller configured it; ``work``
-        alone picks the work dtype (``bf16``, the default, or ``fp32``). Every other keyword goes
-        to ``Engine``: ``slots``, ``page``, ``max_len``, ``pages``, ``prefill_budget``,
+        alone picks the work dtype (``bf16``, the default, or ``fp32``), ``cache="fp8"`` an 8-bit cache of keys and
+        values. Every other keyword goes to ``Engine``: ``slots``, ``page``, ``max_len``, ``pages``, ``prefill_budget``,
         ``graphs``, ``warmup``."""
         self.path = Path(model)
         self._device = torch.device(device)
-        self.model = models.load(model, device, arch or models.configure(model, work=work))
+        self.model = models.load(model, device, arch or models.configure(model, work=work, cache=cache))
         self.tokenizer = self._tokenizer()
         self.eos = folder_stop_ids(self.path)
         self.engine = Engine(self.model, device=device, **engine_kw)

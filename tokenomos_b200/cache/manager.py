@@ -135,7 +135,7 @@ class CacheManager:
                                      f"{g.window}, this spec asks for {spec.window}")
                 g.members.append(key)
                 shape = (num_pages, *spec.page_shape(page_size))
-                self.states[key] = torch.zeros(shape, dtype=dtype, device=self.device)
+                self.states[key] = torch.zeros(shape, dtype=getattr(spec, "dtype", None) or dtype, device=self.device)
                 self.state_groups[key] = spec.group
             elif storage == "slot":
                 self.states[key] = torch.zeros((max_requests + 1, *spec.shape),
@@ -158,13 +158,20 @@ class CacheManager:
         if self.poison:
             for key, spec in specs.items():
                 if spec.storage != "shared" and self.states[key].dtype.is_floating_point:
-                    self.states[key][1:] = float("nan")
+                    rows, nan = self._nan_rows(key)
+                    rows[1:] = nan
 
     def _poison_pages(self, group: Group, pages: list[int]) -> None:
         if pages:
             index = torch.tensor(pages, dtype=torch.long, device=self.device)
             for key in group.members:
-                self.states[key].index_fill_(0, index, float("nan"))
+                rows, nan = self._nan_rows(key)
+                rows.index_fill_(0, index, nan)
+
+    def _nan_rows(self, key: StateKey) -> tuple[torch.Tensor, float | int]:
+        """A state's rows and what fills them with NaN: bytes where the type is an 8-bit one."""
+        t = self.states[key]
+        return (t.view(torch.uint8), 0x7F) if t.dtype.itemsize == 1 else (t, float("nan"))
 
     def _poison_slot(self, slot: int) -> None:
         for key, spec in self.specs.items():
@@ -178,7 +185,7 @@ class CacheManager:
         total = 0
         for key, spec in self.specs.items():
             if spec.storage == "paged":
-                total += math.prod(spec.page_shape(self.page_size)) * self.dtype.itemsize
+                total += math.prod(spec.page_shape(self.page_size)) * (getattr(spec, "dtype", None) or self.dtype).itemsize
         return total
 
     def bytes_per_slot(self) -> int:

@@ -88,6 +88,7 @@ class Engine:
             pages = max(2, min(pages, slots * -(-max_len // page) + 1))
         self.cache = CacheManager(specs, page, pages, slots, model.dtype, self.device, max_len,
                                   poison=poison)
+        self._cache8 = any(t.dtype == ops.KV8_DTYPE for t in self.cache.states.values())
         self.step_fn = StepFunction(model, self.cache)
         self.scheduler = Scheduler(self.cache, prefill_budget, slots)
         # a step is recorded as a CUDA graph only if every part of the model can be (see
@@ -238,7 +239,10 @@ class Engine:
         if self.stats.steps == self._checked_at or self.cache.device.type != "cuda":
             return
         self._checked_at = self.stats.steps
-        for what, where in (("GEMM", ops.gemm_tc_status()), ("attention", ops.attention_prefill_tc_status())):
+        found = [("GEMM", ops.gemm_tc_status()), ("attention", ops.attention_prefill_tc_status())]
+        if self._cache8:
+            found.append(("8-bit cache's attention", ops.attention_kv8_status()))
+        for what, where in found:
             if where:
                 ops.clear_tickets()      # a CTA that gave up may have left its tile's ticket drawn
                 raise RuntimeError(f"a tcgen05 {what} kernel gave up waiting on a barrier (place {where}); "

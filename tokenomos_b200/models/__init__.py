@@ -56,18 +56,25 @@ class Configured:
     arch: object
     config: object
     work: torch.dtype
+    cache: str | None = None
 
 
-def configure(path: str | Path, work: str | torch.dtype | None = None) -> Configured:
+CACHES = (None, "fp8")
+
+
+def configure(path: str | Path, work: str | torch.dtype | None = None, cache: str | None = None) -> Configured:
     """The declaration of folder ``path``'s architecture. ``work``: ``bf16`` (default) or
-    ``fp32``, the storage type of activations, matrices and caches."""
+    ``fp32``, the storage type of activations, matrices and caches. ``cache``: ``fp8`` caches keys and values in 8 bits (e4m3
+    with a power-of-two scale for each page and KV head; softmax attention layers with heads of 64 or 128)."""
+    if cache not in CACHES:
+        raise ValueError(f"cache {cache!r}; known: {CACHES}")
     raw = json.loads((Path(path) / "config.json").read_text("utf-8"))
     arch = architecture_of(raw)
     if isinstance(work, str):
         if work not in WORK_DTYPES:
             raise ValueError(f"work dtype {work!r}; known: {sorted(WORK_DTYPES)}")
         work = WORK_DTYPES[work]
-    return Configured(arch, arch.config_class.from_dict(raw), work or torch.bfloat16)
+    return Configured(arch, arch.config_class.from_dict(raw), work or torch.bfloat16, cache)
 
 
 def load(path: str | Path, device: torch.device | str = "cuda", arch: Configured | None = None,
@@ -78,7 +85,7 @@ def load(path: str | Path, device: torch.device | str = "cuda", arch: Configured
     conf = arch or configure(path)
     ckpt = Checkpoint(path)
     spec = conf.arch.declare(conf.config, ckpt.names())
-    rt = Runtime(conf.work, torch.device(device), tuning or Tuning.for_device(device))
+    rt = Runtime(conf.work, torch.device(device), tuning or Tuning.for_device(device), conf.cache == "fp8")
     tensors = load_tensors(ckpt, spec.tensor_decls(), rt.dtype, rt.device, spec.scope)
     model = build_model(spec, tensors, rt)
     model.config = conf.config
@@ -89,7 +96,7 @@ def load(path: str | Path, device: torch.device | str = "cuda", arch: Configured
 def from_tensors(conf: Configured, tensors: dict, device: torch.device | str = "cuda"):
     """A model from tensors already in memory (the random-weights mode without a folder)."""
     spec = conf.arch.declare(conf.config, tensors.keys())
-    rt = Runtime(conf.work, torch.device(device), Tuning.for_device(device))
+    rt = Runtime(conf.work, torch.device(device), Tuning.for_device(device), conf.cache == "fp8")
     model = build_model(spec, tensors, rt)
     model.config = conf.config
     model.spec = spec

@@ -23,7 +23,7 @@ __all__ = [
     "attention_prefill_tc_status",
     "conv_gated", "conv_min_tile",
     "gemm", "gemm_skinny", "gemm_skinny_conv", "gemm_skinny_ok", "gemm_tc", "gemm_tc_ok", "gemm_tc_status", "sample", "sample_status", "gather_rows_select",
-    "qk_norm_rope_write8", "kv8_supported", "attention_kv8_decode", "attention_kv8_prefill", "attention_kv8_tokens",
+    "KV8_DTYPE", "qk_norm_rope_write8", "kv8_supported", "attention_kv8_decode", "attention_kv8_prefill", "attention_kv8_tokens",
     "attention_kv8_status", "copy_rows",
 ]
 
@@ -1964,6 +1964,6 @@ def attention_biased_mma(q: torch.Tensor, kv_pool: torch.Tensor, out: torch.Tens
 
 
 # the 8-bit cache's operators (they use the helpers above)
-from tokenomos_b200.ops.kv8 import (attention_kv8_decode, attention_kv8_prefill, attention_kv8_status,  # noqa: E402
+from tokenomos_b200.ops.kv8 import (KV8_DTYPE, attention_kv8_decode, attention_kv8_prefill, attention_kv8_status,  # noqa: E402
                                     attention_kv8_tokens, copy_rows,
                                     kv8_supported, qk_norm_rope_write8)

@@ -21,7 +21,8 @@ softmax maps over the same values, each with its own half of the query and of th
 ``a_1 - lambda a_2`` and brought to unit root mean square per head); ``shape`` (``ScoreShape``: the scores' soft cap ``c tanh(s / c)`` and,
 after it, a learned bias by distance); ``chunk`` (in place of a window: a query sees the keys of its own chunk of that many
 positions, counted from the sequence's start, up to its own); ``value_mix`` (``ValueMix``: the cached values are mixed
-with an earlier layer's values of the same token). A position part may keep state per request (a short
+with an earlier layer's values of the same token); ``cache8`` (keys and values are cached in 8 bits, e4m3 with a power-of-two scale
+for each page and KV head, and the softmax runs over what the cache holds, the step's own keys included). A position part may keep state per request (a short
 convolution on q, k and v): it then has ``state_specs()`` and is called with the layer's ``call``.
 """
 
@@ -34,7 +35,7 @@ from dataclasses import dataclass
 import torch
 
 from tokenomos_b200 import ops
-from tokenomos_b200.parts.contract import ChunkKV, HeadLayout, PagedKV, SharedState, StepContext, ValueRows, WindowKV
+from tokenomos_b200.parts.contract import BlockScales, ChunkKV, HeadLayout, PagedKV, SharedState, StepContext, ValueRows, WindowKV
 from tokenomos_b200.parts.linear import Linear
 from tokenomos_b200.parts.registry import DEFAULT_TUNING, Runtime, Tuning, builder_of, register
 
@@ -114,7 +115,7 @@ class Attention:
                  keep_first: int = 0, v_dim: int | None = None, v_is_k: bool = False,
                  gate_kind: str = "head", exact: bool = False, pointwise: PointwiseWeights | None = None,
                  diff: DiffMaps | None = None, shape: ScoreShape | None = None, chunk: int | None = None,
-                 value_mix: ValueMix | None = None):
+                 value_mix: ValueMix | None = None, cache8: bool = False):
         """``gate``: the per-head gate's projection as a part of its own; ``gate_fused``: its rows
         are the last of ``qkv``'s instead (after q, k, v, then zero rows up to a multiple of 8), so
         that one product yields both. With ``diff``, ``heads`` counts the maps (twice the output heads)
@@ -154,6 +155,17 @@ class Attention:
                              "writes them")
         if pointwise is not None and (sink or keep_first):
             raise ValueError("attention: a sink and kept first positions belong to the softmax")
+        self.cache8 = bool(cache8)
+        if cache8:
+            if (pointwise is not None or diff is not None or shape is not None or value_mix is not None or keep_first or v_is_k
+                    or v_dim != head_dim):
+                raise ValueError("attention: an 8-bit cache goes with a plain softmax (a window, chunks and a sink included) over values of "
+                                 "the keys' size")
+            if not ops.kv8_supported(heads, kv_heads, head_dim):
+                raise ValueError(f"attention: an 8-bit cache for {heads} heads over {kv_heads} of {head_dim} (heads of 64 or 128, at most 16 "
+                                 "a KV head)")
+            if not hasattr(rope, "encode_qk8") or (kv_source is None and (q_norm is None) != (k_norm is None)):
+                raise ValueError("attention: an 8-bit cache needs a position part that writes it, and q and k norms both or neither")
         # what the one-kernel decode form and the norms folded into the projections do not take
         # (the tensor-core kernels take all of it but a value size of its own; the general
         # kernel takes everything)
@@ -212,13 +224,20 @@ class Attention:
         # a position part with state of its own per request lists it (under names of its own)
         more = self.rope.state_specs(self.head_layout) if hasattr(self.rope, "state_specs") else {}
         if self.kv_source is not None:
+            if self.cache8:
+                more = {"kv_scale": SharedState(self.kv_source, "kv_scale"), **more}
             return {"kv": SharedState(self.kv_source, "kv"), **more}
         row = max(self.head_dim, self.v_dim)         # a cache row holds a key or a value
+        dtype = ops.KV8_DTYPE if self.cache8 else None
         if self.chunk is not None:
-            return {"kv": ChunkKV(self.kv_heads, row, self.chunk), **more}
-        if self.window is None:
-            return {"kv": PagedKV(self.kv_heads, row), **more}
-        return {"kv": WindowKV(self.kv_heads, row, self.window, self.keep_first), **more}
+            kv = ChunkKV(self.kv_heads, row, self.chunk, dtype)
+        elif self.window is None:
+            kv = PagedKV(self.kv_heads, row, dtype)
+        else:
+            kv = WindowKV(self.kv_heads, row, self.window, self.keep_first, dtype)
+        if self.cache8:
+            more = {"kv_scale": BlockScales(kv), **more}
+        return {"kv": kv, **more}
 
     def forward(self, x: torch.Tensor, ctx: StepContext, call: int) -> torch.Tensor:
         T = x.shape[0]
@@ -278,7 +297,7 @@ class Attention:
     def _fused_decode(self, ctx: StepContext) -> bool:
         """Whether this step's attention runs as one kernel: every sequence brings one token, the
         position encoding is a plain rotation that says so, and the kernel takes the shape."""
-        if not (self.decode_fused and ctx.host.decode_only and self.gate is None
+        if not (self.decode_fused and ctx.host.decode_only and self.gate is None and not self.cache8
                 and ctx.n_tokens <= self.tuning.decode_fused_rows):
             return False
         if self._fused_freqs is None:
@@ -327,6 +346,8 @@ class Attention:
         pool = ctx.states[(call, "kv")]
         table = ctx.block_tables[ctx.state_groups[(call, "kv")]]
         own_kv = self.head_layout.kv_heads
+        if self.cache8:
+            return self._core8(qkv, pool, ctx.states[(call, "kv_scale")], table, ctx, gate)
         if hasattr(self.rope, "state_specs"):
             q = self.rope.encode_qk(qkv, ctx, self.head_layout, pool if own_kv else None,
                                     table if own_kv else None, call=call)
@@ -374,6 +395,28 @@ class Attention:
         if gate is not None and self.gate_kind == "head":
             ops.head_gate(out, gate, self.heads, self.v_dim)
         elif gate is not None:
+            ops.sigmoid_gate(out, gate)
+        return out
+
+    def _core8(self, qkv, pool, scales, table, ctx: StepContext, gate) -> torch.Tensor:
+        """``_core`` over an 8-bit cache: prompt portions in tiles, single tokens with their keys shared out over CTAs."""
+        if self.head_layout.kv_heads:
+            q = self.rope.encode_qk8(qkv, ctx, self.head_layout, pool, scales, table)
+        else:
+            q = self.rope.encode_qk(qkv, ctx, self.head_layout, None, None)
+        out = torch.empty_like(q)
+        by_head = gate if self.gate_kind == "head" else None
+        if not ctx.host.decode_only:
+            per_tile = ops.attention_kv8_tokens(self.heads, self.kv_heads, self.head_dim, ctx.page_size, q.dtype)
+            _, tok0, _, ntok = ctx.tiles(per_tile, "multi")
+            if tok0.numel():
+                ops.attention_kv8_prefill(q, pool, scales, out, ctx.positions, ctx.tok_seq, table, tok0, ntok, self.reach, self.scale,
+                                          ctx.host.longest, by_head, self.sink)
+        singles = None if ctx.host.decode_only else ctx.singles()
+        if singles is None or singles.numel():
+            ops.attention_kv8_decode(q, pool, scales, out, ctx.positions, ctx.tok_seq, table, singles, self.reach, self.scale,
+                                     ctx.host.longest, by_head, self.sink)
+        if gate is not None and by_head is None:
             ops.sigmoid_gate(out, gate)
         return out
 
@@ -666,4 +709,4 @@ def build_attention(params: dict, tensors: dict, rt: Runtime) -> Attention:
         gate_kind=params.get("gate_kind", "head"), exact=params.get("exact", False),
         pointwise=_pointwise(params.get("pointwise"), tensors), diff=_diff(params.get("diff"), tensors),
         shape=_shape(params.get("shape"), tensors, params["heads"], params.get("window")), chunk=params.get("chunk"),
-        value_mix=_value_mix(params.get("value_mix"), tensors))
+        value_mix=_value_mix(params.get("value_mix"), tensors), cache8=rt.cache8)

@@ -39,6 +39,14 @@ def _block(spec: BlockSpec, tensors: dict, rt: Runtime):
     return builder_of("block", spec.kind)(parts)
 
 
+def check_cache8(stack, rt: Runtime) -> None:
+    """Raise unless every paged state of a model that was asked to cache in 8 bits does."""
+    for (call, name), state in stack.state_specs().items() if rt.cache8 else ():
+        if state.storage == "paged" and getattr(state, "dtype", None) is None:
+            raise ValueError(f"an 8-bit cache was asked for, but entry {call} of the layer list keeps its {name!r} in the work dtype: "
+                             "its mixer has no 8-bit form")
+
+
 def build_model(spec: ModelSpec, tensors: dict, rt: Runtime) -> Stack:
     """``tensors``: name -> tensor on ``rt.device``, kept as the weight loader keeps them."""
     blocks = [_block(b, tensors, rt) for b in spec.blocks]
@@ -46,7 +54,9 @@ def build_model(spec: ModelSpec, tensors: dict, rt: Runtime) -> Stack:
     head = Linear(tensors[spec.head.name], tuning=rt.tuning) if spec.head is not None else None
     extras = {name: tensors[decl.name] for name, decl in spec.extras if decl.name in tensors}
     embedder = _part("embedding", spec.embedder, tensors, rt) if spec.embedder is not None else None
-    return Stack(tensors[spec.embedding.name], blocks, list(spec.order), final_norm, head,
-                 tuning=rt.tuning, embed_scale=spec.embed_scale, logit_softcap=spec.logit_softcap,
-                 suppress=spec.suppress, extras=extras, embedder=embedder,
-                 embed_wide=spec.embed_wide, logit_scale=spec.logit_scale)
+    stack = Stack(tensors[spec.embedding.name], blocks, list(spec.order), final_norm, head,
+                  tuning=rt.tuning, embed_scale=spec.embed_scale, logit_softcap=spec.logit_softcap,
+                  suppress=spec.suppress, extras=extras, embedder=embedder,
+                  embed_wide=spec.embed_wide, logit_scale=spec.logit_scale)
+    check_cache8(stack, rt)
+    return stack

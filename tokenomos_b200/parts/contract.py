@@ -26,7 +26,7 @@ bring a spec class of its own: ``storage`` (``"paged"``, ``"slot"`` or ``"shared
 storage ``group`` (specs with equal groups share page numbers and block tables), ``window``
 (None: every position is kept), optionally ``keep_first`` (positions at the start of a sequence
 that a window never passes), ``chunk`` (positions are read chunk by chunk; ``window`` is then a
-chunk's size) and ``page_shape(page_size)`` (the shape of one page); for slot
+chunk's size), ``dtype`` (its storage type; absent or None: the work dtype) and ``page_shape(page_size)`` (the shape of one page); for slot
 storage ``shape`` and ``dtype``; for shared storage ``source`` and ``name``.
 
 Captured steps. With ``graphs=True`` the engine records a step's kernels once per shape and
@@ -49,10 +49,11 @@ import torch
 
 @dataclass(frozen=True)
 class PagedKV:
-    """Keys and values of every position: ``[pages, 2, kv_heads, page, head_dim]``."""
+    """Keys and values of every position: ``[pages, 2, kv_heads, page, head_dim]``. ``dtype`` None = work dtype."""
 
     kv_heads: int
     head_dim: int
+    dtype: torch.dtype | None = None
     storage = "paged"
     window = None
 
@@ -74,6 +75,7 @@ class WindowKV:
     head_dim: int
     window: int
     keep_first: int = 0
+    dtype: torch.dtype | None = None
     storage = "paged"
 
     @property
@@ -92,6 +94,7 @@ class ChunkKV:
     kv_heads: int
     head_dim: int
     chunk: int
+    dtype: torch.dtype | None = None
     storage = "paged"
 
     @property
@@ -104,6 +107,35 @@ class ChunkKV:
 
     def page_shape(self, page_size: int) -> tuple[int, ...]:
         return (2, self.kv_heads, page_size, self.head_dim)
+
+
+@dataclass(frozen=True)
+class BlockScales:
+    """One float32 for each block of an 8-bit cache's pages (keys or values of a page, one KV head): ``[pages, 2, kv_heads]``.
+    It lies with the pages of ``of``: the same group, windows and chunks."""
+
+    of: "PagedKV | WindowKV | ChunkKV"
+    storage = "paged"
+    dtype = torch.float32
+
+    @property
+    def group(self) -> tuple:
+        return self.of.group
+
+    @property
+    def window(self) -> int | None:
+        return self.of.window
+
+    @property
+    def keep_first(self) -> int:
+        return getattr(self.of, "keep_first", 0)
+
+    @property
+    def chunk(self) -> int:
+        return getattr(self.of, "chunk", 0)
+
+    def page_shape(self, page_size: int) -> tuple[int, ...]:
+        return (2, self.of.kv_heads)
 
 
 @dataclass(frozen=True)
@@ -143,7 +175,7 @@ class SharedState:
 
 
 # the specs the framework's own parts use; any object with the attributes above is one too
-StateSpec = PagedKV | WindowKV | ChunkKV | LatentKV | SlotState | SharedState
+StateSpec = PagedKV | WindowKV | ChunkKV | BlockScales | LatentKV | SlotState | SharedState
 # the "call" under which the state of a model's embedding part is keyed (it is no entry of the
 # layer list)
 EMBED_CALL = -1

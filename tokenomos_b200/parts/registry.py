@@ -104,11 +104,13 @@ DEFAULT_TUNING = Tuning()
 @dataclass(frozen=True)
 class Runtime:
     """What every part is built for: the work dtype (storage of activations, matrices and
-    caches), the device, and the device's kernel-choice thresholds."""
+    caches), the device, the device's kernel-choice thresholds, and whether keys and values are cached in 8 bits
+    (``cache8``: a part that keeps paged keys and values and has no such form refuses)."""
 
     dtype: torch.dtype
     device: torch.device
     tuning: Tuning = DEFAULT_TUNING
+    cache8: bool = False
 
 
 Builder = Callable[[dict, dict, Runtime], object]

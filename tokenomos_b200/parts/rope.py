@@ -47,6 +47,13 @@ class Rope:
             heads.head_dim, ctx.page_size)
 
 
+    def encode_qk8(self, qkv: torch.Tensor, ctx: StepContext, heads: HeadLayout, pool: torch.Tensor, scales: torch.Tensor,
+                   table: torch.Tensor) -> torch.Tensor:
+        """``encode_qk`` for an 8-bit cache (cos and sin, and everything before the quantisation, stay 32-bit)."""
+        return ops.qk_norm_rope_write8(qkv, pool, scales, heads.q_norm, heads.k_norm, heads.eps, self.inv_freq, ctx.positions,
+                                       ctx.tok_seq, table, heads.heads, heads.kv_heads, heads.head_dim, ctx.page_size)
+
+
 @register("position", "rope")
 def build_rope(params: dict, tensors: dict, rt: Runtime) -> Rope:
     return Rope(params["head_dim"], params["angles"], params["theta"], rt.device,
@@ -118,6 +125,14 @@ class Rotary:
                                 heads.heads, heads.kv_heads, heads.head_dim,
                                 heads.v_dim if heads.v_dim is not None else heads.head_dim, ctx.page_size,
                                 self.interleaved, heads.v_is_k)
+
+
+    def encode_qk8(self, qkv: torch.Tensor, ctx: StepContext, heads: HeadLayout, pool: torch.Tensor, scales: torch.Tensor,
+                   table: torch.Tensor) -> torch.Tensor:
+        """``encode_qk`` for an 8-bit cache."""
+        return ops.qk_norm_rope_write8(qkv, pool, scales, heads.q_norm, heads.k_norm, heads.eps, self.freq, ctx.positions,
+                                       ctx.tok_seq, table, heads.heads, heads.kv_heads, heads.head_dim, ctx.page_size,
+                                       self.cs_mult, self.interleaved)
 
 
 @register("position", "rotary")
