@@ -441,8 +441,29 @@ TK_API int tk_attn_kv8_supported(int H, int Hkv, int D) {
     return Hkv > 0 && H > 0 && H % Hkv == 0 && H / Hkv <= K8_ROWS && (D == 64 || D == 128);
 }
 
+// Whether prompt portions of this shape take the tcgen05 kernel: 16-bit, heads of 64, a group that divides 128, pages that are a power of two and 16 or more
+// positions.
+TK_API int tk_attn_kv8_prefill_supported(int H, int Hkv, int D, int P, int dtype) {
+    return tk_attn_kv8_supported(H, Hkv, D) && dtype == TK_BF16 && D == 64 && 128 % (H / Hkv) == 0 && P >= 16 && (P & (P - 1)) == 0;
+}
+
 // Tokens of one sequence a tile of tk_attn_kv8 has.
-TK_API int tk_attn_kv8_tokens(int H, int Hkv) { return K8_ROWS / (H / Hkv); }
+TK_API int tk_attn_kv8_tokens(int H, int Hkv, int D, int P, int dtype) {
+    return (tk_attn_kv8_prefill_supported(H, Hkv, D, P, dtype) ? 128 : K8_ROWS) / (H / Hkv);
+}
+
+// The most CTAs (1, 2, 4 or 8, a cluster) that may share one tile's keys in the tcgen05 kernel for portions, for a step of `tokens` tokens in tiles of
+// 128 / G whose list has `items` entries (a captured step's is longer than what it uses): doubled while each keeps 8 key tiles, the CTAs are
+// two an SM at most, and from two on, beyond one an SM, only where each keeps 32 (two CTAs of an SM walk at 0.7 of one's pace).
+TK_API int tk_attn_kv8_prefill_splits(int tokens, int items, int H, int Hkv, int longest, int sm_count) {
+    const int per_tile = 128 / (H / Hkv);
+    const int64_t ctas = (int64_t)((tokens + per_tile - 1) / per_tile) * Hkv, launched = (int64_t)items * Hkv;
+    int split = 1;
+    while (split < 8 && 2 * split * ctas <= 2 * (int64_t)sm_count && 2 * split * launched <= 2048 && longest >= 2 * split * 480 &&
+           (split == 1 || 2 * split * ctas <= sm_count || longest >= split * 2048))
+        split *= 2;
+    return split;
+}
 
 // Ways to share the keys of each of `items` tiles out over CTAs, when no sequence holds more than `longest` positions and a query sees at most `reach` of them. tc:
 // single tokens through the tcgen05 kernel: as many as keep every CTA resident (four an SM for heads of 64 with up to four query heads a KV head, else two: one
@@ -473,14 +494,15 @@ TK_API int tk_attn_kv8_single_tc(int P, int dtype) { return dtype == TK_BF16 && 
 
 int tk_attn_kv8_tc(const void* q, const void* pool, const float* scales, void* out, const void* args, int D, cudaStream_t stream);
 int tk_attn_kv8_tc_status();
+int tk_attn_kv8_prefill_tc(const void* q, const void* pool, const float* scales, void* out, const void* args, cudaStream_t stream);
+int tk_attn_kv8_prefill_tc_status();
 
 // 0, or 1 if a warp gave up waiting for its keys since the last call. Resets the word.
 TK_API int tk_attn_kv8_status() {
-    int v = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&v, g_k8_error, sizeof(int)) != cudaSuccess) return -1;
-    if (v != 0) cudaMemcpyToSymbol(g_k8_error, &zero, sizeof(int));
-    const int tc = tk_attn_kv8_tc_status();
-    return v != 0 ? v : tc;
+    const int found[3] = {k8_take_status(), tk_attn_kv8_tc_status(), tk_attn_kv8_prefill_tc_status()};
+    for (int v : found)
+        if (v != 0) return v;
+    return 0;
 }
 
 // q, out: [T, H, D]; pool: [pages, 2, Hkv, P, D] bytes, scales: [pages, 2, Hkv]. item_tok0 / item_ntok: tiles of at most tk_attn_kv8_tokens tokens of one
@@ -492,7 +514,8 @@ TK_API int tk_attn_kv8(const void* q, const void* pool, const float* scales, voi
                        cudaStream_t stream) {
     TK_CHECK_ARG(tk_attn_kv8_supported(H, Hkv, D), "attn_kv8: shape H=%d Hkv=%d D=%d is not taken (heads of 64 or 128, up to %d a KV head)", H,
                  Hkv, D, K8_ROWS);
-    TK_CHECK_ARG(items >= 0 && P > 0 && nsplit >= 1 && (nsplit == 1 || scratch != nullptr || (item_ntok == nullptr && tk_attn_kv8_single_tc(P, dtype))), "attn_kv8: bad sizes");
+    const bool meets_in_scratch = item_ntok == nullptr ? !tk_attn_kv8_single_tc(P, dtype) : !tk_attn_kv8_prefill_supported(H, Hkv, D, P, dtype);
+    TK_CHECK_ARG(items >= 0 && P > 0 && nsplit >= 1 && (nsplit == 1 || scratch != nullptr || !meets_in_scratch), "attn_kv8: bad sizes");
     TK_CHECK_ARG(item_ntok == nullptr || item_tok0 != nullptr, "attn_kv8: tiles have first tokens");
     TK_CHECK_ARG((int64_t)items * Hkv * nsplit < 0x7fffffff, "attn_kv8: %d splits of %d items", nsplit, items);
     TK_CHECK_ARG(scale > 0.f, "attn_kv8: the scores' factor is positive");
@@ -505,6 +528,10 @@ TK_API int tk_attn_kv8(const void* q, const void* pool, const float* scales, voi
     const int G = H / Hkv;
     K8Args a{positions, tok_seq, block_table, item_tok0, item_ntok, gate, scratch, ldg, bt_stride, items, H, Hkv, P, shift, window, nsplit, sink,
              item_ntok != nullptr ? (K8_ROWS / G) * G : G, scale};
+    if (item_ntok != nullptr && tk_attn_kv8_prefill_supported(H, Hkv, D, P, dtype)) {
+        TK_CHECK_ARG(nsplit == 1 || nsplit == 2 || nsplit == 4 || nsplit == 8, "attn_kv8: %d shares of a tile's keys (1, 2, 4 or 8)", nsplit);
+        return tk_attn_kv8_prefill_tc(q, pool, scales, out, &a, stream);
+    }
     if (item_ntok == nullptr && tk_attn_kv8_single_tc(P, dtype)) {
         TK_CHECK_ARG(nsplit <= 16, "attn_kv8: %d shares of a token's keys (at most 16)", nsplit);
         return tk_attn_kv8_tc(q, pool, scales, out, &a, D, stream);

@@ -27,7 +27,7 @@
 #include <math.h>
 
 #include "kv8_attn.cuh"
-#include "tcgen05.cuh"
+#include "kv8_tc.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -38,47 +38,6 @@ constexpr int K8T_COPIERS = 2;                             // warps that bring k
 constexpr int K8T_MMA_WARP = 4 + K8T_COPIERS, K8T_THREADS = (K8T_MMA_WARP + 1) * 32;
 constexpr int K8T_PTERMS = 4;
 constexpr float K8T_LAZY = 2.0f, K8T_LIFT = 6.0f, K8T_FINE = 256.0f;
-
-// K-major or MN-major operand whose rows are D = 64 (64-byte swizzle) or 128 bytes (128-byte swizzle), groups of eight rows one after the other
-template <int BYTES>
-__device__ __forceinline__ uint64_t desc8(uint32_t at) {
-    uint64_t d = 0;
-    d |= (uint64_t)((at & 0x3FFFF) >> 4);
-    d |= (uint64_t)1 << 16;
-    d |= (uint64_t)((8 * BYTES) >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)(BYTES == 64 ? 4 : 2) << 61;
-    return d;
-}
-// byte offset of 16-byte chunk `chunk` of row `row`
-template <int BYTES>
-__device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
-    return (uint32_t)(row * BYTES + ((BYTES == 64 ? chunk ^ ((row >> 1) & 3) : chunk ^ (row & 7)) << 4));
-}
-
-// e4m3 x e4m3 -> f32
-__host__ __device__ constexpr uint32_t idesc8(int m, int n, bool a_m_major) {
-    return (1u << 4) | (a_m_major ? 1u << 15 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-
-__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-__device__ __forceinline__ bool elect_lane() {
-    uint32_t mine;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "elect.sync _|p, 0xffffffff;\n\t"
-        "selp.b32 %0, 1, 0, p;\n\t}"
-        : "=r"(mine));
-    return mine != 0;
-}
 
 // eight columns of this thread's lane; the loads of several calls are waited for together
 __device__ __forceinline__ void tmem_ld8_start(uint32_t addr, uint32_t* r) {
@@ -497,19 +456,6 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
     }
 }
 
-// the cache as rows of D bytes, boxes of a page or of 128 positions of one
-bool k8t_map(CUtensorMap* map, const void* pool, int D, int P) {
-    EncodeTiled fn = encode_fn();
-    if (fn == nullptr) return false;
-    const cuuint64_t dims[2] = {(cuuint64_t)D, 0x7fffffffu};
-    const cuuint64_t strides[1] = {(cuuint64_t)D};
-    const cuuint32_t box[2] = {(cuuint32_t)D, (cuuint32_t)(P < K8T_KEYS ? P : K8T_KEYS)};
-    const cuuint32_t estr[2] = {1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(pool), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int D, int NR>
 cudaError_t k8t_launch(const void* q, const float* scales, void* out, const CUtensorMap& map, const K8Args& a, cudaStream_t stream) {
     constexpr int smem = K8tSmem<D, NR>::BYTES;
@@ -522,19 +468,8 @@ cudaError_t k8t_launch(const void* q, const float* scales, void* out, const CUte
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
-    int n = 0;
-    if (tk_pdl_enabled()) {
-        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[n++].val.programmaticStreamSerializationAllowed = 1;
-    }
-    if (a.nsplit > 1) {
-        attr[n].id = cudaLaunchAttributeClusterDimension;
-        attr[n].val.clusterDim.x = (unsigned)a.nsplit;
-        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
-        ++n;
-    }
     cfg.attrs = attr;
-    cfg.numAttrs = n;
+    cfg.numAttrs = k8_attributes(attr, a.nsplit);
     return cudaLaunchKernelEx(&cfg, attn_kv8_tc_kernel<D, NR>, (const __nv_bfloat16*)q, scales, (__nv_bfloat16*)out, map, a);
 }
 
@@ -553,7 +488,7 @@ cudaError_t k8t_rows(const void* q, const float* scales, void* out, const CUtens
 int tk_attn_kv8_tc(const void* q, const void* pool, const float* scales, void* out, const void* args, int D, cudaStream_t stream) {
     const K8Args& a = *static_cast<const K8Args*>(args);
     CUtensorMap map = {};
-    TK_CHECK_ARG(k8t_map(&map, pool, D, a.P), "attn_kv8: cuTensorMapEncodeTiled failed");
+    TK_CHECK_ARG(k8_map(&map, pool, D, a.P < K8T_KEYS ? a.P : K8T_KEYS), "attn_kv8: cuTensorMapEncodeTiled failed");
     const cudaError_t e = D == 64 ? k8t_rows<64>(q, scales, out, map, a, stream) : k8t_rows<128>(q, scales, out, map, a, stream);
     if (e != cudaSuccess) {
         tk_set_error("attn_kv8: launch failed: %s", cudaGetErrorString(e));
@@ -563,9 +498,4 @@ int tk_attn_kv8_tc(const void* q, const void* pool, const float* scales, void* o
     return 0;
 }
 
-int tk_attn_kv8_tc_status() {
-    int v = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&v, g_k8_error, sizeof(int)) != cudaSuccess) return -1;
-    if (v != 0) cudaMemcpyToSymbol(g_k8_error, &zero, sizeof(int));
-    return v;
-}
+int tk_attn_kv8_tc_status() { return k8_take_status(); }

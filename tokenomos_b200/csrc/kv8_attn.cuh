@@ -47,6 +47,14 @@ __device__ __forceinline__ bool k8_wait(uint32_t bar, uint32_t parity) {
     return true;
 }
 
+// 0, or 1 if a wait of this file's kernels gave up since the last call; -1: the word could not be read
+inline int k8_take_status() {
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_k8_error, sizeof(int)) != cudaSuccess) return -1;
+    if (v != 0) cudaMemcpyToSymbol(g_k8_error, &zero, sizeof(int));
+    return v;
+}
+
 struct K8Args {
     const int* positions;
     const int* tok_seq;

@@ -16,7 +16,7 @@ import torch
 
 from tokenomos_b200 import ops
 from tokenomos_b200.ops import _lib
-from tokenomos_b200.ops._lib import BF16, KernelError
+from tokenomos_b200.ops._lib import BF16, F32, KernelError
 
 KV8_DTYPE = torch.float8_e4m3fn
 
@@ -110,18 +110,21 @@ def _sms(device: torch.device) -> int:
     return n
 
 
-def _attend(q, pool, scales, out, positions, tok_seq, block_table, tok0, ntok, items, rows, shape, window, scale, longest, gate, sink):
+def _attend(q, pool, scales, out, positions, tok_seq, block_table, tok0, ntok, items, nsplit, rows, shape, window, scale, gate, sink):
+    """``rows`` > 0: the shares of a tile (of so many rows) meet in scratch memory."""
     T, H, Hkv, P, D, code = shape
-    reach = abs(int(window)) + rows - 1 if window else longest
-    tc = ntok is None and code == BF16 and P >= 16 and not P & (P - 1)
-    nsplit = _lib.call("tk_attn_kv8_splits", items, H, Hkv, D, int(longest), reach, _sms(q.device), tc)
     scratch = None
-    if nsplit > 1 and not tc:
-        scratch = torch.empty(items * Hkv * nsplit * rows * (H // Hkv) * (D + 4), dtype=torch.float32, device=q.device)
+    if nsplit > 1 and rows:
+        scratch = torch.empty(items * Hkv * nsplit * rows * (D + 4), dtype=torch.float32, device=q.device)
     _lib.call("tk_attn_kv8", q.data_ptr(), pool.data_ptr(), scales.data_ptr(), out.data_ptr(), positions.data_ptr(), tok_seq.data_ptr(),
               block_table.data_ptr(), block_table.stride(0), ops._ptr(tok0), ops._ptr(ntok), items, H, Hkv, D, P, int(window or 0),
               float(scale), nsplit, ops._ptr(scratch), ops._ptr(gate), gate.stride(0) if gate is not None else 0, int(bool(sink)), code,
               ops._stream())
+
+
+def _whole_pages(P: int) -> bool:
+    """Whether pages are a power of two and 16 positions or more, as the tcgen05 kernels take them."""
+    return P >= 16 and not P & (P - 1)
 
 
 def attention_kv8_decode(q: torch.Tensor, pool: torch.Tensor, scales: torch.Tensor, out: torch.Tensor, positions: torch.Tensor,
@@ -137,12 +140,16 @@ def attention_kv8_decode(q: torch.Tensor, pool: torch.Tensor, scales: torch.Tens
     _here(name, tok_index)
     n = shape[0] if tok_index is None else ops._i32(tok_index, "tok_index").numel()
     if n:
-        _attend(q, pool, scales, out, positions, tok_seq, block_table, tok_index, None, n, 1, shape, window, scale, longest, gate, sink)
+        T, H, Hkv, P, D, code = shape
+        tc = code == BF16 and _whole_pages(P)
+        nsplit = _lib.call("tk_attn_kv8_splits", n, H, Hkv, D, int(longest), abs(int(window)) if window else int(longest), _sms(q.device), tc)
+        _attend(q, pool, scales, out, positions, tok_seq, block_table, tok_index, None, n, nsplit, 0 if tc else H // Hkv, shape, window, scale,
+                gate, sink)
 
 
 def attention_kv8_tokens(heads: int, kv_heads: int, head_dim: int, page: int, dtype: torch.dtype) -> int:
     """The most tokens of one sequence that a tile of ``attention_kv8_prefill`` has."""
-    return _lib.call("tk_attn_kv8_tokens", heads, kv_heads)
+    return _lib.call("tk_attn_kv8_tokens", heads, kv_heads, head_dim, page, F32 if dtype == torch.float32 else BF16)
 
 
 def attention_kv8_prefill(q: torch.Tensor, pool: torch.Tensor, scales: torch.Tensor, out: torch.Tensor, positions: torch.Tensor,
@@ -152,14 +159,20 @@ def attention_kv8_prefill(q: torch.Tensor, pool: torch.Tensor, scales: torch.Ten
     """The same for prompt portions: tiles of at most ``attention_kv8_tokens`` tokens of one sequence at consecutive positions (``tile_tok0``:
     each one's first row of ``q``; ``tile_ntok``: its tokens, 0 for an unused entry); writes the tiles' rows of ``out``."""
     name = "attention_kv8_prefill"
-    shape = T, H, Hkv, P, D, code = _check_attention(name, q, pool, scales, out, positions, tok_seq, block_table, gate)
+    T, H, Hkv, P, D, code = shape = _check_attention(name, q, pool, scales, out, positions, tok_seq, block_table, gate)
     _here(name, tile_tok0, tile_ntok)
     n = ops._i32(tile_tok0, "tile_tok0").numel()
     if ops._i32(tile_ntok, "tile_ntok").numel() != n:
         raise KernelError(f"{name}: {n} first tokens for {tile_ntok.numel()} tiles")
     if n:
-        rows = _lib.call("tk_attn_kv8_tokens", H, Hkv)
-        _attend(q, pool, scales, out, positions, tok_seq, block_table, tile_tok0, tile_ntok, n, rows, shape, window, scale, longest, gate, sink)
+        reach = min(int(longest), abs(int(window)) + T) if window else int(longest)
+        rows = 0
+        if _lib.call("tk_attn_kv8_prefill_supported", H, Hkv, D, P, code):
+            nsplit = _lib.call("tk_attn_kv8_prefill_splits", T, n, H, Hkv, reach, _sms(q.device))
+        else:
+            rows = _lib.call("tk_attn_kv8_tokens", H, Hkv, D, P, code) * (H // Hkv)
+            nsplit = _lib.call("tk_attn_kv8_splits", n, H, Hkv, D, reach, reach, _sms(q.device), 0)
+        _attend(q, pool, scales, out, positions, tok_seq, block_table, tile_tok0, tile_ntok, n, nsplit, rows, shape, window, scale, gate, sink)
 
 
 def attention_kv8_status() -> int:
