@@ -6,7 +6,8 @@
 // recorded launch keeps what it was recorded with. Bound by HBM (each byte read and written once) or, for a few pages, by
 // the launch; a CTA moves 16 KB, four 16-byte loads of a thread in flight.
 #include <algorithm>
-#include <vector>
+#include <memory>
+#include <new>
 
 #include "common.cuh"
 
@@ -99,19 +100,29 @@ TK_API int tk_copy_rows(void* const* base, const int64_t* row, const int* rows, 
     for (int i = 0; i < pairs; ++i)
         TK_CHECK_ARG(src[i] >= 0 && src[i] < least && dst[i] >= 0 && dst[i] < least, "copy_rows: row %d to %d, outside 0..%d", src[i],
                      dst[i], least - 1);
-    if (pairs > 1 || src[0] == dst[0]) {
-        try {
-            std::vector<int> to(dst, dst + pairs);
-            std::sort(to.begin(), to.end());
-            for (int i = 1; i < pairs; ++i)
-                TK_CHECK_ARG(to[i] != to[i - 1], "copy_rows: row %d is a destination twice", to[i]);
-            for (int i = 0; i < pairs; ++i)
-                TK_CHECK_ARG(!std::binary_search(to.begin(), to.end(), src[i]), "copy_rows: row %d is both a source and a destination", src[i]);
-        } catch (...) {
+    // no destination twice, none that is a source: a bit a row (a few pairs are compared with each other)
+    int twice = -1, both = -1;
+    if (pairs <= 16) {
+        for (int i = 0; i < pairs; ++i)
+            for (int j = 0; j < pairs; ++j) {
+                if (j < i && dst[i] == dst[j]) twice = dst[i];
+                if (src[i] == dst[j]) both = src[i];
+            }
+    } else {
+        std::unique_ptr<uint64_t[]> seen(new (std::nothrow) uint64_t[(size_t)least / 64 + 1]());
+        if (!seen) {
             tk_set_error("copy_rows: no memory to check %d pairs", pairs);
             return -3;
         }
+        for (int i = 0; i < pairs; ++i) {
+            if (seen[dst[i] >> 6] >> (dst[i] & 63) & 1) twice = dst[i];
+            seen[dst[i] >> 6] |= 1ull << (dst[i] & 63);
+        }
+        for (int i = 0; i < pairs; ++i)
+            if (seen[src[i] >> 6] >> (src[i] & 63) & 1) both = src[i];
     }
+    TK_CHECK_ARG(twice < 0, "copy_rows: row %d is a destination twice", twice);
+    TK_CHECK_ARG(both < 0, "copy_rows: row %d is both a source and a destination", both);
     if (pairs <= 16) return copy_some<32, 16>(base, row, tensors, src, dst, pairs, stream);
     return copy_some<32, 1024>(base, row, tensors, src, dst, pairs, stream);
 }

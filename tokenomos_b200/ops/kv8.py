@@ -9,7 +9,6 @@ head). A byte stands for ``scale * e4m3``; a block's scale is the smallest with 
 from __future__ import annotations
 
 import array
-import ctypes
 from typing import Sequence
 
 import torch
@@ -23,29 +22,34 @@ KV8_DTYPE = torch.float8_e4m3fn
 
 def _here(name: str, *tensors: torch.Tensor | None) -> None:
     """Every tensor on the current device, whose stream the launch goes to."""
-    ops._cuda(*tensors)
-    now = torch.cuda.current_device()
+    found = -1
     for t in tensors:
-        if t is not None and t.device.index != now:
-            raise KernelError(f"{name}: a tensor on {t.device} while cuda:{now} is the current device")
+        if t is not None:
+            device = t.get_device()
+            if device < 0:
+                ops._cuda(t)
+            if found < 0:
+                found = torch._C._cuda_getDevice()
+            if device != found:
+                raise KernelError(f"{name}: a tensor on {t.device} while cuda:{found} is the current device")
 
 
 def _check_cache(name: str, pool: torch.Tensor, scales: torch.Tensor) -> tuple[int, int, int]:
     """(kv_heads, page, head_dim) of an 8-bit cache."""
-    if pool.dtype != KV8_DTYPE or pool.dim() != 5 or pool.shape[1] != 2 or not pool.is_contiguous():
+    shape = pool.shape
+    if len(shape) != 5 or pool.dtype != KV8_DTYPE or shape[1] != 2 or not pool.is_contiguous():
         raise KernelError(f"{name}: the cache is a contiguous {KV8_DTYPE} [pages, 2, kv_heads, page, head_dim] tensor, "
-                          f"got {pool.dtype} {tuple(pool.shape)}")
-    if scales.dtype != torch.float32 or scales.shape != pool.shape[:3] or not scales.is_contiguous():
-        raise KernelError(f"{name}: the scales are a contiguous float32 {tuple(pool.shape[:3])} tensor, got "
+                          f"got {pool.dtype} {tuple(shape)}")
+    if scales.dtype != torch.float32 or scales.shape != shape[:3] or not scales.is_contiguous():
+        raise KernelError(f"{name}: the scales are a contiguous float32 {tuple(shape[:3])} tensor, got "
                           f"{scales.dtype} {tuple(scales.shape)}")
-    return pool.shape[2], pool.shape[3], pool.shape[4]
+    return shape[2], shape[3], shape[4]
 
 
 def _check_layout(name: str, tokens: int, positions: torch.Tensor, tok_seq: torch.Tensor, block_table: torch.Tensor) -> None:
-    for what, t in (("positions", positions), ("tok_seq", tok_seq)):
-        if ops._i32(t, what).numel() < tokens:
-            raise KernelError(f"{name}: {what} is shorter than the {tokens} rows")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+    if ops._i32(positions, "positions").numel() < tokens or ops._i32(tok_seq, "tok_seq").numel() < tokens:
+        raise KernelError(f"{name}: positions or tok_seq is shorter than the {tokens} rows")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
         raise KernelError(f"{name}: block_table is an int32 [sequences, blocks] tensor with contiguous rows")
 
 
@@ -85,14 +89,15 @@ def qk_norm_rope_write8(qkv: torch.Tensor, pool: torch.Tensor, scales: torch.Ten
     return q
 
 
-def _check_attention(name, q, pool, scales, out, positions, tok_seq, block_table, gate):
-    _here(name, q, pool, scales, out, positions, tok_seq, block_table, gate)
+def _check_attention(name, q, pool, scales, out, positions, tok_seq, block_table, gate, *lists):
+    _here(name, q, pool, scales, out, positions, tok_seq, block_table, gate, *lists)
     Hkv, P, D = _check_cache(name, pool, scales)
-    if (q.dim() != 3 or q.shape[2] != D or q.shape[1] % Hkv or out.shape != q.shape or out.dtype != q.dtype
+    shape, dtype = q.shape, q.dtype
+    if (len(shape) != 3 or shape[2] != D or shape[1] % Hkv or out.shape != shape or out.dtype != dtype
             or not (q.is_contiguous() and out.is_contiguous())):
-        raise KernelError(f"{name}: contiguous q and out [T, H, {D}] of one type, H a multiple of {Hkv}; got {tuple(q.shape)} "
-                          f"{q.dtype} and {tuple(out.shape)} {out.dtype}")
-    T, H, _ = q.shape
+        raise KernelError(f"{name}: contiguous q and out [T, H, {D}] of one type, H a multiple of {Hkv}; got {tuple(shape)} "
+                          f"{dtype} and {tuple(out.shape)} {out.dtype}")
+    T, H, _ = shape
     code = ops._dtype_code(q)
     _check_layout(name, T, positions, tok_seq, block_table)
     if gate is not None and (gate.dtype != q.dtype or tuple(gate.shape) != (T, H) or gate.stride(1) != 1):
@@ -103,7 +108,7 @@ def _check_attention(name, q, pool, scales, out, positions, tok_seq, block_table
 _sm_count: dict = {}
 
 
-def _sms(device: torch.device) -> int:
+def _sms(device: int) -> int:
     n = _sm_count.get(device)
     if n is None:
         n = _sm_count[device] = torch.cuda.get_device_properties(device).multi_processor_count
@@ -136,13 +141,12 @@ def attention_kv8_decode(q: torch.Tensor, pool: torch.Tensor, scales: torch.Tens
     a row's keys are shared out. ``gate`` [T, H]: the per-head output gate, ``round(o) * round(sigmoid(gate))``; ``sink``: the
     softmax's denominator has one term more, a key of score 0 without a value."""
     name = "attention_kv8_decode"
-    shape = _check_attention(name, q, pool, scales, out, positions, tok_seq, block_table, gate)
-    _here(name, tok_index)
+    shape = _check_attention(name, q, pool, scales, out, positions, tok_seq, block_table, gate, tok_index)
     n = shape[0] if tok_index is None else ops._i32(tok_index, "tok_index").numel()
     if n:
         T, H, Hkv, P, D, code = shape
         tc = code == BF16 and _whole_pages(P)
-        nsplit = _lib.call("tk_attn_kv8_splits", n, H, Hkv, D, int(longest), abs(int(window)) if window else int(longest), _sms(q.device), tc)
+        nsplit = _lib.call("tk_attn_kv8_splits", n, H, Hkv, D, int(longest), abs(int(window)) if window else int(longest), _sms(q.get_device()), tc)
         _attend(q, pool, scales, out, positions, tok_seq, block_table, tok_index, None, n, nsplit, 0 if tc else H // Hkv, shape, window, scale,
                 gate, sink)
 
@@ -159,8 +163,7 @@ def attention_kv8_prefill(q: torch.Tensor, pool: torch.Tensor, scales: torch.Ten
     """The same for prompt portions: tiles of at most ``attention_kv8_tokens`` tokens of one sequence at consecutive positions (``tile_tok0``:
     each one's first row of ``q``; ``tile_ntok``: its tokens, 0 for an unused entry); writes the tiles' rows of ``out``."""
     name = "attention_kv8_prefill"
-    T, H, Hkv, P, D, code = shape = _check_attention(name, q, pool, scales, out, positions, tok_seq, block_table, gate)
-    _here(name, tile_tok0, tile_ntok)
+    T, H, Hkv, P, D, code = shape = _check_attention(name, q, pool, scales, out, positions, tok_seq, block_table, gate, tile_tok0, tile_ntok)
     n = ops._i32(tile_tok0, "tile_tok0").numel()
     if ops._i32(tile_ntok, "tile_ntok").numel() != n:
         raise KernelError(f"{name}: {n} first tokens for {tile_ntok.numel()} tiles")
@@ -168,10 +171,10 @@ def attention_kv8_prefill(q: torch.Tensor, pool: torch.Tensor, scales: torch.Ten
         reach = min(int(longest), abs(int(window)) + T) if window else int(longest)
         rows = 0
         if _lib.call("tk_attn_kv8_prefill_supported", H, Hkv, D, P, code):
-            nsplit = _lib.call("tk_attn_kv8_prefill_splits", T, n, H, Hkv, reach, _sms(q.device))
+            nsplit = _lib.call("tk_attn_kv8_prefill_splits", T, n, H, Hkv, reach, _sms(q.get_device()))
         else:
             rows = _lib.call("tk_attn_kv8_tokens", H, Hkv, D, P, code) * (H // Hkv)
-            nsplit = _lib.call("tk_attn_kv8_splits", n, H, Hkv, D, reach, reach, _sms(q.device), 0)
+            nsplit = _lib.call("tk_attn_kv8_splits", n, H, Hkv, D, reach, reach, _sms(q.get_device()), 0)
         _attend(q, pool, scales, out, positions, tok_seq, block_table, tile_tok0, tile_ntok, n, nsplit, rows, shape, window, scale, gate, sink)
 
 
@@ -185,20 +188,23 @@ def copy_rows(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence
     requests' state rows. ``src`` and ``dst`` are host integers; no row is a destination twice, and none both a source and a
     destination (refused)."""
     _here("copy_rows", *tensors)
-    for t in tensors:
-        if t.dim() < 1 or not t.is_contiguous():
-            raise KernelError("copy_rows: contiguous tensors whose first dimension counts the rows")
     if len(src) != len(dst):
         raise KernelError(f"copy_rows: {len(src)} sources for {len(dst)} destinations")
-    tensors = [t for t in tensors if t.numel()]
-    if not tensors or not len(src):
+    base, row, rows = [], [], []
+    for t in tensors:
+        shape, size = t.shape, t.nbytes
+        if not shape or not t.is_contiguous():
+            raise KernelError("copy_rows: contiguous tensors whose first dimension counts the rows")
+        if size:
+            base.append(t.data_ptr())
+            row.append(size // shape[0])
+            rows.append(shape[0])
+    if not base or not len(src):
         return
     try:
         a, b = array.array("i", src), array.array("i", dst)
     except (TypeError, OverflowError) as exc:
         raise KernelError(f"copy_rows: rows are numbered by 32-bit integers ({exc})") from None
-    n = len(tensors)
-    base = (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors])
-    row = (ctypes.c_int64 * n)(*[t.stride(0) * t.element_size() if t.shape[0] > 1 else t.numel() * t.element_size() for t in tensors])
-    rows = (ctypes.c_int * n)(*[t.shape[0] for t in tensors])
-    _lib.call("tk_copy_rows", base, row, rows, n, a.buffer_info()[0], b.buffer_info()[0], len(a), ops._stream())
+    base, row, rows = array.array("Q", base), array.array("q", row), array.array("i", rows)
+    _lib.call("tk_copy_rows", base.buffer_info()[0], row.buffer_info()[0], rows.buffer_info()[0], len(rows), a.buffer_info()[0],
+              b.buffer_info()[0], len(a), ops._stream())
