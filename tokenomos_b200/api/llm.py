@@ -116,22 +116,31 @@ class LLM:
 
     def request(self, ids: list[int], p: SamplingParams) -> Request:
         """The engine request for one prompt: ``p``'s options, and as stops the folder's
-        end-of-sequence ids followed by ``p.stop_token_ids`` (each id once)."""
+        end-of-sequence ids followed by ``p.stop_token_ids`` (each id once). With ``p.n`` > 1 the request for its first reply, the others
+        its ``siblings``."""
         p.validate()
         stops = list(self.eos)
         stops.extend(t for t in p.stop_token_ids if t not in stops)
-        return Request(prompt=list(ids), max_new=p.max_tokens, temperature=p.temperature,
-                       top_p=p.top_p, top_k=p.top_k, min_p=p.min_p, seed=p.seed, stop=tuple(stops))
+        first, *others = (Request(prompt=list(ids), max_new=p.max_tokens, temperature=p.temperature, top_p=p.top_p, top_k=p.top_k,
+                                  min_p=p.min_p, seed=p.seed + i, stop=tuple(stops)) for i in range(p.n))
+        first.siblings = others
+        return first
 
     def submit(self, req: Request) -> Future:
         """Hand ``req`` to the engine. The future's result is ``req`` itself, with ``result``
         filled in, as soon as the engine has finished it. A request the engine can never serve
         raises here, in the caller's thread."""
+        return self.submit_all(req)[0]
+
+    def submit_all(self, req: Request) -> list[Future]:
+        """``submit`` with the futures of ``req`` and of its ``siblings``, in order."""
         self._check_worker()
-        done: Future = Future()
-        req.on_done = done.set_result
+        futs = []
+        for r in (req, *req.siblings):
+            futs.append(Future())
+            r.on_done = futs[-1].set_result
         self.engine.submit(req)
-        return done
+        return futs
 
     def wait(self, futs: list[Future]) -> list[Request]:
         """The finished requests behind ``futs``, in their order. Raises ``RuntimeError`` (with
@@ -155,16 +164,19 @@ class LLM:
     # ---- many ----
 
     def generate(self, prompts: list, params: SamplingParams | None = None) -> list[Output]:
-        """One reply per prompt, in order. A prompt is a list of token ids, or text."""
+        """One reply per prompt, in order, or ``params.n`` side by side. A prompt is a list of token ids, or text."""
         params = params or SamplingParams()
-        futs = [self.submit(self.request(self._ids(prompt), params)) for prompt in prompts]
+        futs = [fut for prompt in prompts for fut in self.submit_all(self.request(self._ids(prompt), params))]
         return [self.output(req) for req in self.wait(futs)]
 
     def stream(self, prompt, params: SamplingParams | None = None):
         """Yields the reply's token ids in runs, as the engine delivers them (the host reads a
         step's tokens while the next step runs). The runs joined are ``generate``'s reply."""
+        params = params or SamplingParams()
+        if params.n != 1:
+            raise ValueError(f"stream: one reply, not {params.n}")
         runs: queue.Queue = queue.Queue()
-        req = self.request(self._ids(prompt), params or SamplingParams())
+        req = self.request(self._ids(prompt), params)
         req.on_tokens = lambda toks: runs.put(list(toks))
         fut = self.submit(req)
         while True:

@@ -8,7 +8,9 @@ every layer of the group indexes its own tensor ``[pages, 2, kv_heads, page, hea
 the group's page numbers. Pages return to the group's pool when the request ends, or, in a
 window group, as soon as no later query can see them (the pages of a group's kept first
 positions stay to the end), and are handed out again (lowest number
-first, so runs are reproducible). Page 0 of every pool and slot 0 are never handed out: padded
+first, so runs are reproducible). A request may be forked: its copies share the pages that are full (each page goes back when the last
+request that holds it lets it go), and get pages of their own for the one being filled, which is copied together with
+the state rows. Page 0 of every pool and slot 0 are never handed out: padded
 rows of a batch point there. Fixed-size state (``SlotState``) is a row ``[*shape]`` per request
 in a ``[slots, *shape]`` tensor; a request starting at position 0 reads it as zeros by
 contract, so rows are not cleared on reuse.
@@ -22,6 +24,7 @@ from __future__ import annotations
 
 import heapq
 import math
+from collections import Counter
 from dataclasses import dataclass, field
 
 import torch
@@ -38,13 +41,15 @@ class CacheError(RuntimeError):
 
 
 class FreeList:
-    """Numbers ``first .. count-1``, handed out lowest first, each held at most once."""
+    """Numbers ``first .. count-1``, handed out lowest first; one that is held may be shared, and is free again when all who
+    hold it have given it back."""
 
     def __init__(self, count: int, first: int = 1):
         self.count, self.first = count, first
         self._heap = list(range(first, count))
         heapq.heapify(self._heap)
         self._held: set[int] = set()
+        self._more: dict[int, int] = {}         # holders beyond the first, of the numbers that are shared
 
     def __len__(self) -> int:
         return len(self._heap)
@@ -56,11 +61,29 @@ class FreeList:
         self._held.add(n)
         return n
 
-    def give(self, n: int) -> None:
+    def give(self, n: int) -> bool:
+        """One holder lets ``n`` go; whether that frees it."""
         if n not in self._held:
             raise CacheError(f"{n} given back but not held (freed twice, or never taken)")
+        more = self._more.get(n, 0)
+        if more:
+            if more == 1:
+                del self._more[n]
+            else:
+                self._more[n] = more - 1
+            return False
         self._held.remove(n)
         heapq.heappush(self._heap, n)
+        return True
+
+    def share(self, n: int) -> None:
+        """One holder more for ``n``."""
+        if n not in self._held:
+            raise CacheError(f"{n} shared but not held")
+        self._more[n] = self._more.get(n, 0) + 1
+
+    def holders(self, n: int) -> int:
+        return self._more.get(n, 0) + 1 if n in self._held else 0
 
     @property
     def held(self) -> set[int]:
@@ -307,11 +330,11 @@ class CacheManager:
             passed = min(self._first_needed_block(g, st.length), len(table))
             # the blocks of the kept first positions are never passed
             start = max(st.first_live.get(k, 0), -(-g.keep_first // self.page_size))
-            if self.poison:
-                self._poison_pages(g, [table[b] for b in range(start, passed)])
+            freed = [table[b] for b in range(start, passed) if g.pages.give(table[b])]
             for b in range(start, passed):
-                g.pages.give(table[b])
                 table[b] = 0
+            if self.poison:
+                self._poison_pages(g, freed)
             st.first_live[k] = max(st.first_live.get(k, 0), passed)
 
     def release(self, rid) -> None:
@@ -320,14 +343,60 @@ class CacheManager:
         if st is None:
             raise CacheError(f"request {rid!r} is not live (released twice?)")
         for k, g in self.groups.items():
-            for page in st.tables[k]:
-                if page:
-                    g.pages.give(page)
+            freed = [page for page in st.tables[k] if page and g.pages.give(page)]
             if self.poison:
-                self._poison_pages(g, [page for page in st.tables[k] if page])
+                self._poison_pages(g, freed)
         if self.poison:
             self._poison_slot(st.slot)
         self.slots.give(st.slot)
+
+    # ---- forks ----
+
+    def fork_pages(self, rid) -> int:
+        """Pages that a copy of ``rid`` takes from each group: one if its last page is partly filled."""
+        return 1 if self._get(rid).length % self.page_size else 0
+
+    def fork(self, rid, children: list) -> list[RequestState]:
+        """Admit ``children`` (request ids) as copies of ``rid`` at its present length, all or nothing: full pages are shared, the page
+        being filled and the state rows are copied on the device (in stream order: behind the steps that were queued before)."""
+        st = self._get(rid)
+        taken = [c for c in children if c in self.requests]
+        if taken or len(set(children)) != len(children):
+            raise CacheError(f"requests {taken or children!r} are already live")
+        full, part = divmod(st.length, self.page_size)
+        if len(self.slots) < len(children) or (part and self.free_pages() < len(children)):
+            raise OutOfPages(f"{len(children)} forks of request {rid!r} need a slot each" + (" and a page of each group" if part else ""))
+        copies: list[RequestState] = []
+        for child in children:
+            new = self.admit(child)
+            new.length = new.reserved = st.length
+            new.first_live = dict(st.first_live)
+            for k, g in self.groups.items():
+                table = st.tables[k][:full]
+                for page in table:
+                    if page:
+                        g.pages.share(page)
+                new.tables[k] = table + ([g.pages.take()] if part else [])
+            if self.groups:
+                new.held_tokens = min(len(t) for t in new.tables.values()) * self.page_size
+            copies.append(new)
+        if part and copies:
+            for k, g in self.groups.items():
+                self._copy_rows([self.states[m] for m in g.members], [st.tables[k][full]] * len(copies), [new.tables[k][full] for new in copies])
+        rows = [self.states[key] for key, spec in self.specs.items() if spec.storage == "slot"]
+        if rows and copies and st.length:
+            self._copy_rows(rows, [st.slot] * len(copies), [new.slot for new in copies])
+        return copies
+
+    def _copy_rows(self, tensors: list, src: list[int], dst: list[int]) -> None:
+        if self.device.type == "cuda":
+            from tokenomos_b200 import ops
+
+            ops.copy_rows(tensors, src, dst)
+        elif self.device.type != "meta":
+            for t in tensors:
+                raw = t.view(torch.uint8) if t.dtype.itemsize == 1 else t
+                raw[dst] = raw[src]
 
     def _get(self, rid) -> RequestState:
         st = self.requests.get(rid)
@@ -347,11 +416,11 @@ class CacheManager:
     # ---- invariants (tests call this after every operation) ----
 
     def check(self) -> None:
-        """No page lost, none held twice: per group, pages held by requests and free pages
-        partition ``1 .. num_pages-1``; same for slots."""
+        """No page lost, none held by others than the books say: per group, pages held by requests (a shared one by as many as share
+        it) and free pages partition ``1 .. num_pages-1``; same for slots."""
         for k, g in self.groups.items():
             held = [p for st in self.requests.values() for p in st.tables[k] if p]
-            if len(held) != len(set(held)):
+            if len(held) != sum(g.pages.holders(p) for p in set(held)) or any(n != g.pages.holders(p) for p, n in Counter(held).items()):
                 raise CacheError(f"group {k}: a page is held twice")
             if set(held) != g.pages.held:
                 raise CacheError(f"group {k}: pages held by requests differ from the pool's books")

@@ -20,7 +20,11 @@ Pages run out (decided here, tested in tests/test_scheduler.py):
    (The reference lets the newest rows sit out with their state intact instead,
    core/engine.py:843-858; recomputing needs no pages held by idle rows.)
 
-The scheduler owns no device memory and runs no kernel: ``plan`` returns what to run,
+Several replies of one prompt (``Request.siblings``): the first request reads the prompt up to its last token, then its cache is
+forked for the others (``CacheManager.fork``: full pages are shared), and each runs the last token and its own reply like any
+other request. A sibling that finds no slot or pages at that moment waits like any other request, and reads the prompt itself.
+
+The scheduler owns no device memory and runs no kernel (but a fork's copies): ``plan`` returns what to run,
 ``commit`` takes the sampled tokens. Both are plain host code.
 """
 
@@ -59,6 +63,8 @@ class Request:
     result: object = None
     # tokens sampled on the device whose values the host has not read yet (a step in flight)
     inflight: int = 0
+    # requests with the same prompt that are to be forked from this one's cache once it has read all but the prompt's last token
+    siblings: list["Request"] = field(default_factory=list)
 
     @property
     def tokens(self) -> list[int]:
@@ -119,7 +125,7 @@ class Scheduler:
         self.running: list[Request] = []          # in admission order (oldest first)
         self._ids = itertools.count()
         self._arrivals = itertools.count()
-        self.stats = {"steps": 0, "preemptions": 0, "admitted": 0, "finished": 0}
+        self.stats = {"steps": 0, "preemptions": 0, "admitted": 0, "finished": 0, "forked": 0}
 
     # ---- requests in ----
 
@@ -139,12 +145,27 @@ class Scheduler:
         held = (cache.num_pages - 1) * cache.page_size
         if total > held:
             raise ValueError(f"request needs {total} tokens of the {held} the page pool holds")
+        for other in req.siblings:
+            if other.prompt != req.prompt or other.siblings:
+                raise ValueError("siblings have the prompt of the request that they are forked from, and none of their own")
+            self.check(other)
 
     def add(self, req: Request) -> None:
         self.check(req)
-        req.rid = next(self._ids)
-        req.arrival = next(self._arrivals)
+        for r in (req, *req.siblings):
+            r.rid = next(self._ids)
+            r.arrival = next(self._arrivals)
         self.waiting.append(req)
+        if len(req.prompt) == 1:                  # nothing to share
+            self._part(req)
+
+    def _part(self, req: Request, first: bool = False) -> None:
+        """``req``'s siblings go their own way: into the queue, at its front if ``first``."""
+        if first:
+            self.waiting.extendleft(reversed(req.siblings))
+        else:
+            self.waiting.extend(req.siblings)
+        req.siblings = []
 
     def idle(self) -> bool:
         return not self.waiting and not self.running
@@ -173,9 +194,27 @@ class Scheduler:
     def inflight(self) -> bool:
         return any(r.inflight for r in self.running)
 
+    def _fork_siblings(self, req: Request) -> None:
+        """``req`` has read all but its prompt's last token: as many siblings as slots and pages allow become running requests at the
+        same place; the others wait."""
+        cache = self.cache
+        own = self._pages_for(len(req.prompt) + 1) - req.computed // cache.page_size       # pages that a copy does not share
+        room = min(len(req.siblings), self.max_seqs - len(self.running), cache.free_slots(),
+                   max(0, cache.free_pages() - self._outstanding()) // own)
+        now, req.siblings = req.siblings[:room], req.siblings[room:]
+        if now:
+            cache.fork(req.rid, [r.rid for r in now])
+            for r in now:
+                r.computed = req.computed
+            self.running.extend(now)
+            self.stats["forked"] += len(now)
+        self._part(req, first=True)
+
     def plan(self) -> list[Planned]:
         """Decide the next step and hold its pages (``CacheManager.extend``)."""
         cache, budget = self.cache, self.token_budget
+        for req in [r for r in self.running if r.siblings and r.computed == len(r.prompt) - 1]:
+            self._fork_siblings(req)
         planned: list[Planned] = []
         # 1 and 2: running requests, oldest first; a decoding one takes one token, one still
         # reading its prompt a portion of what is left of the budget. Victims are always the
@@ -189,6 +228,8 @@ class Scheduler:
                 break
             total = len(req.prompt) + len(req.output) + req.inflight
             count = min(total - req.computed, budget)
+            if req.siblings:                      # (they are forked before the prompt's last token)
+                count = min(count, len(req.prompt) - 1 - req.computed)
             if count <= 0 or len(req.output) + req.inflight >= req.max_new:
                 # nothing left to compute: its last token is sampled (in flight until the next
                 # delivery), and the cache entry of a token nobody will follow is never read
@@ -220,7 +261,7 @@ class Scheduler:
                 break
             self.waiting.popleft()
             cache.admit(req.rid)
-            count = min(req.pending, budget)
+            count = min(req.pending - bool(req.siblings), budget)
             cache.extend(req.rid, count)
             self.running.append(req)
             self.stats["admitted"] += 1

@@ -6,7 +6,7 @@ declaration and the engine (Tokenomos api/server.py:211-228, bench/decode.py:32-
         --max-tokens 16 --temperature 0.8 --seed 3 --arch-kw '{"work": "bf16"}' \\
         --engine-kw '{"page": 16, "max_len": 512}'
 
-Prints one JSON object per prompt: ``{"prompt_tokens": n, "token_ids": [...], "finish": ...,
+Prints one JSON object per reply (one a prompt, or ``--n``): ``{"prompt_tokens": n, "token_ids": [...], "finish": ...,
 "text": ...}``. ``--random-weights CONFIG.json`` first writes a model folder with random weights
 at ``--model`` from that configuration and ``--seed-weights``.
 """
@@ -32,6 +32,7 @@ def main(argv: list[str] | None = None) -> int:
     ap.add_argument("--top-k", type=int, default=0)
     ap.add_argument("--min-p", type=float, default=0.0)
     ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--n", type=int, default=1, help="replies of each prompt, the i-th with seed + i")
     ap.add_argument("--stop-token-ids", default="", help="comma-separated token ids")
     ap.add_argument("--arch-kw", default="{}", help='JSON kwargs of the declaration, e.g. {"work": "fp32"}')
     ap.add_argument("--engine-kw", default="{}", help="JSON kwargs of the engine")
@@ -57,7 +58,7 @@ def main(argv: list[str] | None = None) -> int:
         ap.error("give at least one --prompt-ids or --prompt")
     stops = tuple(int(t) for t in args.stop_token_ids.split(",") if t.strip())
     params = SamplingParams(args.max_tokens, args.temperature, args.top_p, args.top_k, args.min_p,
-                            args.seed, stops)
+                            args.seed, stops, args.n)
     arch = models.configure(args.model, **json.loads(args.arch_kw))
     with LLM(args.model, args.device, arch, **json.loads(args.engine_kw)) as llm:
         for out in llm.generate(prompts, params):

@@ -17,6 +17,8 @@ class SamplingParams:
     min_p: float = 0.0
     seed: int = 0
     stop_token_ids: tuple[int, ...] = ()
+    # replies of each prompt, the i-th with seed + i; the prompt is read once and its cache forked
+    n: int = 1
 
     def validate(self) -> None:
         if self.max_tokens < 1:
@@ -27,5 +29,7 @@ class SamplingParams:
             raise ValueError(f"top_p {self.top_p} outside (0, 1]")
         if self.top_k < 0:
             raise ValueError(f"top_k {self.top_k} is negative")
+        if self.n < 1:
+            raise ValueError(f"n {self.n}: a prompt has at least one reply")
         if not 0.0 <= self.min_p < 1.0:
             raise ValueError(f"min_p {self.min_p} outside [0, 1)")
