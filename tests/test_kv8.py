@@ -343,7 +343,7 @@ def check_attention(cache, new, H, dtype, window=None, scale=None, sink=False, s
 
 
 SHAPES = [(1, 1, 64, 16), (4, 2, 64, 16), (32, 8, 64, 16), (6, 2, 64, 16), (5, 1, 64, 5), (16, 1, 64, 64), (8, 8, 64, 1), (4, 1, 128, 16),
-          (12, 4, 128, 12), (16, 1, 128, 8), (2, 2, 128, 32), (9, 1, 64, 48)]
+          (12, 4, 128, 12), (16, 1, 128, 8), (2, 2, 128, 32), (9, 1, 64, 48), (4, 2, 64, 128), (8, 1, 64, 256), (4, 1, 128, 256), (8, 4, 64, 32)]
 
 
 @gpu
@@ -460,6 +460,32 @@ def test_a_row_that_sees_nothing_is_zero():
     for sink in (False, True):
         ops.attention_kv8_decode(q, cache.pool, cache.scales, out, i32([-1, 39]), i32([0, 0]), cache.table_dev, None, None, 0.125, 40, None, sink)
         assert (out[0] == 0).all() and torch.isfinite(out[1]).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_tile_longer_than_it_may_be_writes_only_its_own_rows(dtype):
+    lens, H, G, D = [300], 4, 2, 64
+    cache = Cache(lens, G, D, 16).fill()
+    q = torch.randn(300, H, D, generator=torch.Generator().manual_seed(0)).to(dtype).cuda()
+    size = ops.attention_kv8_tokens(H, G, D, 16, dtype)
+    want, pos = run_attention(cache, q, [300], None, 0.125)
+    out = torch.full_like(q, 7.0)
+    ops.attention_kv8_prefill(q, cache.pool, cache.scales, out, pos, i32([0] * 300), cache.table_dev, i32([0]), i32([size + 40]), None, 0.125, 300)
+    assert ((out[:size].float() - want[:size].float()).abs() <= 1e-2).all() and (out[size:] == 7).all()
+
+
+@gpu
+def test_tokens_without_a_position_write_nothing():
+    cache = Cache([16], 2, 64, 16)
+    x = torch.randn(3, 6 * 64, device="cuda")
+    q = ops.qk_norm_rope_write8(x, cache.pool, cache.scales, None, None, 0.0, torch.zeros(0, device="cuda"), i32([-1, 0, 1]), i32([0, 0, 0]), cache.table_dev,
+                                2, 2, 64, 16)
+    assert torch.equal(q, x.view(3, 6, 64)[:, :2])
+    raw = cache.pool.view(torch.uint8)
+    page = int(cache.table[0, 0])
+    assert (raw[page, :, :, :2] != NAN_BYTE).any() and (raw[page, :, :, 2:] == NAN_BYTE).all()
+    assert all((raw[p] == NAN_BYTE).all() for p in range(raw.shape[0]) if p != page)
 
 
 @gpu

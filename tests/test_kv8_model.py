@@ -229,3 +229,30 @@ def test_a_mixer_that_keeps_latents_is_refused():
     with pytest.raises(ValueError, match="no 8-bit form"):
         b.check_cache8(Stack({(0, "kv"): LatentKV(80)}), Runtime(torch.float32, torch.device("cpu"), cache8=True))
     b.check_cache8(Stack({(0, "kv"): LatentKV(80)}), Runtime(torch.float32, torch.device("cpu")))
+
+
+CHECKED = """
+import sys
+sys.path.insert(0, "tests")
+import torch
+import test_kv8_model, trace_util
+from tokenomos_b200 import ops
+folder, dtype = sys.argv[1], sys.argv[2]
+assert ops.checks_enabled()
+g = torch.Generator().manual_seed(3)
+reqs = {f"r{i}": torch.randint(0, 400, (n,), generator=g).tolist() for i, n in enumerate((2, 31, 150, 65, 200))}
+steps = trace_util.mixed(reqs, live=4, seed=7)
+pages = -(-trace_util.max_live_tokens(steps, 16) // 16) + 1
+got = test_kv8_model.replay(*test_kv8_model.engine_of(folder, dtype, 16, pages)[:0:-1], steps)
+assert all(torch.isfinite(v).all() for v in got.values())
+assert ops.checks_status() is None, ops.checks_status()
+print("clean")
+"""
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_replay_under_the_index_checks_finds_nothing(dtype, folders):
+    from test_checks import run_checked
+
+    assert run_checked(CHECKED, str(folders["D"]), dtype).startswith("clean")

@@ -51,7 +51,7 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
 // T: type of q and the output. D: head size. PAGE16: pages are a multiple of 16 positions and a power of two, so 16 keys that begin at a multiple of
 // 16 lie in one page; otherwise every lane looks its own keys' pages up.
 template <typename T, int D, bool PAGE16>
-__global__ void __launch_bounds__(K8_THREADS, D == 64 && sizeof(T) == 2 && PAGE16 ? 4 : 2)
+__global__ void __launch_bounds__(K8_THREADS, D == 64 && PAGE16 ? (sizeof(T) == 2 ? 4 : 3) : 2)
 attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, const K8Args a) {
     constexpr bool WIDE = sizeof(T) == 4;                // q and the weights as two float16
     constexpr int U = D == 64 ? 2 : 1;                   // groups of 16 keys a warp takes at a time
@@ -66,7 +66,7 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
     const int g = lane >> 2, c = lane & 3;
     const int split = blockIdx.x % a.nsplit, kvh = (blockIdx.x / a.nsplit) % a.Hkv, item = blockIdx.x / (a.nsplit * a.Hkv);
     const int tok0 = a.item_tok0 != nullptr ? a.item_tok0[item] : item;
-    const int ntok = a.item_ntok != nullptr ? a.item_ntok[item] : 1;
+    const int ntok = a.item_ntok != nullptr ? min(a.item_ntok[item], K8_ROWS / (a.H / a.Hkv)) : 1;       // (a longer tile's rest is left alone)
     if (tok0 < 0 || ntok <= 0) return;                   // a padded entry of a recorded step
     const int G = a.H / a.Hkv, rows = ntok * G;
     const int* bt = a.block_table + (size_t)a.tok_seq[tok0] * a.bt_stride;

@@ -83,7 +83,7 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
     // the KV head fastest and the tiles in reverse: a causal tile late in its sequence reads the most keys, so the longest CTAs start first
     const int which = blockIdx.x / max_split, kvh = which % Hkv;
     const int tile = gridDim.x / (max_split * Hkv) - 1 - which / Hkv;
-    const int tok0 = a.item_tok0[tile], ntok = a.item_ntok[tile];
+    const int tok0 = a.item_tok0[tile], ntok = min(a.item_ntok[tile], KP_ROWS / G);      // (a longer tile's rest is left alone)
     if (ntok <= 0) return;       // an unused entry of a fixed-length tile list (captured steps); the whole cluster's
     const int rows = ntok * G;
     const int* bt_row = a.block_table + (size_t)a.tok_seq[tok0] * a.bt_stride;

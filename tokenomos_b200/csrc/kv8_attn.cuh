@@ -100,7 +100,7 @@ attn_kv8_merge_kernel(T* out, const K8Args a, float lift) {
     if (item >= a.items) return;
     const int tok0 = a.item_tok0 != nullptr ? a.item_tok0[item] : (int)item;
     const int ntok = a.item_ntok != nullptr ? a.item_ntok[item] : 1;
-    if (tok0 < 0 || r >= ntok * G) return;
+    if (tok0 < 0 || r >= ntok * G) return;               // (r is below a tile's most rows)
     const float* part = a.scratch + ((item * a.Hkv + kvh) * a.nsplit * a.rows_most + r) * (D + 4);
     const size_t step = (size_t)a.rows_most * (D + 4);
     float m_all = -INFINITY;

@@ -212,6 +212,7 @@ qk_norm_rope_write8_kernel(const T* qkv, int64_t qkv_stride, T* q_out, uint8_t* 
         if (on >> j & 1) continue;
         const int t = t_first + j - 1;
         const int pos = __shfl_sync(0xffffffffu, pos_mine, j), seq = __shfl_sync(0xffffffffu, seq_mine, j), off = pos % a.P;
+        if (pos < 0) continue;                            // (no position: nothing is written)
         int n = j < 31 ? __ffs(~(on >> (j + 1))) : 1;     // the run's tokens, as far as these lanes reach
         for (bool more = j + n == 32; more;) {
             const int i = n + lane;

@@ -40,6 +40,8 @@ def _check_cache(name: str, pool: torch.Tensor, scales: torch.Tensor) -> tuple[i
     if len(shape) != 5 or pool.dtype != KV8_DTYPE or shape[1] != 2 or not pool.is_contiguous():
         raise KernelError(f"{name}: the cache is a contiguous {KV8_DTYPE} [pages, 2, kv_heads, page, head_dim] tensor, "
                           f"got {pool.dtype} {tuple(shape)}")
+    if shape[0] * 2 * shape[2] * shape[3] >= 1 << 31:
+        raise KernelError(f"{name}: a cache of {tuple(shape)} has more rows than 31 bits count")
     if scales.dtype != torch.float32 or scales.shape != shape[:3] or not scales.is_contiguous():
         raise KernelError(f"{name}: the scales are a contiguous float32 {tuple(shape[:3])} tensor, got "
                           f"{scales.dtype} {tuple(scales.shape)}")
@@ -67,7 +69,7 @@ def qk_norm_rope_write8(qkv: torch.Tensor, pool: torch.Tensor, scales: torch.Ten
     position. ``inv_freq`` [R / 2]: the first R columns are rotated, pairs (i, i + R / 2), or (2i, 2i + 1) when
     ``interleaved``; cos and sin are multiplied by ``cs_mult``. Everything is 32-bit (angles 64-bit) and rounded once.
 
-    A sequence's tokens lie side by side in the step, at consecutive positions, and a page that tokens are written into
+    A sequence's tokens lie side by side in the step, at consecutive positions (negative ones are not written), and a page that tokens are written into
     belongs to one sequence. A block that already holds tokens of earlier steps keeps its scale or raises it, and then its earlier bytes are
     rounded to the new one (which changes nothing above 2^-6 of it, e4m3's smallest normal number)."""
     name = "qk_norm_rope_write8"
@@ -205,6 +207,6 @@ def copy_rows(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence
         a, b = array.array("i", src), array.array("i", dst)
     except (TypeError, OverflowError) as exc:
         raise KernelError(f"copy_rows: rows are numbered by 32-bit integers ({exc})") from None
-    base, row, rows = array.array("Q", base), array.array("q", row), array.array("i", rows)
+    base, row, rows = array.array("Q", base), array.array("q", row), array.array("i", [min(n, 0x7FFFFFFF) for n in rows])
     _lib.call("tk_copy_rows", base.buffer_info()[0], row.buffer_info()[0], rows.buffer_info()[0], len(rows), a.buffer_info()[0],
               b.buffer_info()[0], len(a), ops._stream())

@@ -33,6 +33,7 @@ def main(argv: list[str] | None = None) -> int:
                     help="most tokens live requests hold at any time (sizes the page pool)")
     ap.add_argument("--page-size", type=int, default=16, help="tokens per cache page")
     ap.add_argument("--max-requests", type=int, default=4, help="live requests (state slots)")
+    ap.add_argument("--cache", choices=["fp8"], help="cache keys and values in 8 bits")
     ap.add_argument("--device", default="cuda:0")
     args = ap.parse_args(argv)
 
@@ -50,7 +51,7 @@ def main(argv: list[str] | None = None) -> int:
     ops.available()
     out = Path(args.out)
     out.mkdir(parents=True, exist_ok=True)
-    conf = models.configure(args.model, work=args.dtype)
+    conf = models.configure(args.model, work=args.dtype, cache=args.cache)
     model = models.load(args.model, args.device, conf)
     page = args.page_size
     pages = -(-args.max_tokens // page) + 1          # + the null page
