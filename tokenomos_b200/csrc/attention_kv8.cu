@@ -441,10 +441,10 @@ TK_API int tk_attn_kv8_supported(int H, int Hkv, int D) {
     return Hkv > 0 && H > 0 && H % Hkv == 0 && H / Hkv <= K8_ROWS && (D == 64 || D == 128);
 }
 
-// Whether prompt portions of this shape take the tcgen05 kernel: 16-bit, heads of 64, a group that divides 128, pages that are a power of two and 16 or more
+// Whether prompt portions of this shape take the tcgen05 kernel: 16-bit, a group that divides 128, pages that are a power of two and 16 or more
 // positions.
 TK_API int tk_attn_kv8_prefill_supported(int H, int Hkv, int D, int P, int dtype) {
-    return tk_attn_kv8_supported(H, Hkv, D) && dtype == TK_BF16 && D == 64 && 128 % (H / Hkv) == 0 && P >= 16 && (P & (P - 1)) == 0;
+    return tk_attn_kv8_supported(H, Hkv, D) && dtype == TK_BF16 && 128 % (H / Hkv) == 0 && P >= 16 && (P & (P - 1)) == 0;
 }
 
 // Tokens of one sequence a tile of tk_attn_kv8 has.
@@ -454,12 +454,12 @@ TK_API int tk_attn_kv8_tokens(int H, int Hkv, int D, int P, int dtype) {
 
 // The most CTAs (1, 2, 4 or 8, a cluster) that may share one tile's keys in the tcgen05 kernel for portions, for a step of `tokens` tokens in tiles of
 // 128 / G whose list has `items` entries (a captured step's is longer than what it uses): doubled while each keeps 8 key tiles, the CTAs are
-// two an SM at most, and from two on, beyond one an SM, only where each keeps 32 (two CTAs of an SM walk at 0.7 of one's pace).
-TK_API int tk_attn_kv8_prefill_splits(int tokens, int items, int H, int Hkv, int longest, int sm_count) {
+// two an SM at most (heads of 128: one, as many as find room), and from two on, beyond one an SM, only where each keeps 32 (two CTAs of an SM walk at 0.7 of one's pace).
+TK_API int tk_attn_kv8_prefill_splits(int tokens, int items, int H, int Hkv, int D, int longest, int sm_count) {
     const int per_tile = 128 / (H / Hkv);
     const int64_t ctas = (int64_t)((tokens + per_tile - 1) / per_tile) * Hkv, launched = (int64_t)items * Hkv;
     int split = 1;
-    while (split < 8 && 2 * split * ctas <= 2 * (int64_t)sm_count && 2 * split * launched <= 2048 && longest >= 2 * split * 480 &&
+    while (split < 8 && 2 * split * ctas <= (D == 64 ? 2 : 1) * (int64_t)sm_count && 2 * split * launched <= 2048 && longest >= 2 * split * 480 &&
            (split == 1 || 2 * split * ctas <= sm_count || longest >= split * 2048))
         split *= 2;
     return split;
@@ -494,7 +494,7 @@ TK_API int tk_attn_kv8_single_tc(int P, int dtype) { return dtype == TK_BF16 && 
 
 int tk_attn_kv8_tc(const void* q, const void* pool, const float* scales, void* out, const void* args, int D, cudaStream_t stream);
 int tk_attn_kv8_tc_status();
-int tk_attn_kv8_prefill_tc(const void* q, const void* pool, const float* scales, void* out, const void* args, cudaStream_t stream);
+int tk_attn_kv8_prefill_tc(const void* q, const void* pool, const float* scales, void* out, const void* args, int D, cudaStream_t stream);
 int tk_attn_kv8_prefill_tc_status();
 
 // 0, or 1 if a warp gave up waiting for its keys since the last call. Resets the word.
@@ -530,7 +530,7 @@ TK_API int tk_attn_kv8(const void* q, const void* pool, const float* scales, voi
              item_ntok != nullptr ? (K8_ROWS / G) * G : G, scale};
     if (item_ntok != nullptr && tk_attn_kv8_prefill_supported(H, Hkv, D, P, dtype)) {
         TK_CHECK_ARG(nsplit == 1 || nsplit == 2 || nsplit == 4 || nsplit == 8, "attn_kv8: %d shares of a tile's keys (1, 2, 4 or 8)", nsplit);
-        return tk_attn_kv8_prefill_tc(q, pool, scales, out, &a, stream);
+        return tk_attn_kv8_prefill_tc(q, pool, scales, out, &a, D, stream);
     }
     if (item_ntok == nullptr && tk_attn_kv8_single_tc(P, dtype)) {
         TK_CHECK_ARG(nsplit <= 16, "attn_kv8: %d shares of a token's keys (at most 16)", nsplit);

@@ -1,4 +1,4 @@
-// Prompt portions' attention over the 8-bit cache (kv8.cuh) on the fifth-generation tensor cores, for bfloat16 and heads of 64.
+// Prompt portions' attention over the 8-bit cache (kv8.cuh) on the fifth-generation tensor cores, for bfloat16.
 //
 //   S  = q K^T     tcgen05.mma kind::f8f6f4, M = 128 rows, N = 64 keys: K's bytes as they land, q as two e4m3 terms (attention_kv8_tc.cu)
 //                  multiplied one after the other into the same accumulator
@@ -32,22 +32,28 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int KP_D = 64, KP_ROWS = 128, KP_KEYS = 64, KP_GROUPS = KP_KEYS / 16;
+constexpr int KP_ROWS = 128, KP_KEYS = 64, KP_GROUPS = KP_KEYS / 16;
 constexpr int KP_THREADS = 384;
 constexpr int KP_STAGES = 5;
-constexpr int KP_Q_BYTES = KP_ROWS * KP_D;                 // of a term
-constexpr int KP_RAW = KP_KEYS * KP_D;                     // keys' or values' bytes of a tile
-constexpr int KP_V16 = KP_KEYS * KP_D * 2;
-constexpr int KP_Q = 0, KP_K = 2 * KP_Q_BYTES, KP_V = KP_K + KP_STAGES * KP_RAW, KP_H = KP_V + KP_STAGES * KP_RAW;
-constexpr int KP_SCALES = KP_H + KP_STAGES * KP_V16;       // [stage][group] (key's, value's)
-constexpr int KP_FACTOR = KP_SCALES + KP_STAGES * KP_GROUPS * 8;
-constexpr int KP_BARS = KP_FACTOR + KP_ROWS * 4;
-constexpr int KP_SMEM = KP_BARS + (3 * KP_STAGES + 7) * 8 + 16;
-constexpr int KP_SHARE_LD = KP_D + 4;
 constexpr int KP_SPLIT_TILES = 8;                          // key tiles a CTA should have before a tile's keys are shared out
 constexpr float KP_LAZY = 8.0f, KP_LIFT = 7.0f;
-static_assert(KP_K % 1024 == 0 && KP_V % 1024 == 0 && KP_H % 1024 == 0 && KP_SCALES % 8 == 0, "swizzled tiles");
-static_assert(KP_ROWS * (KP_SHARE_LD + 2) * 4 <= KP_SCALES - KP_K, "a share of the keys lies where the tiles were");
+
+// shared memory of a CTA: two fit an SM for heads of 64, one for heads of 128
+template <int D>
+struct KpSmem {
+    static constexpr int Q_BYTES = KP_ROWS * D;            // of a term
+    static constexpr int RAW = KP_KEYS * D;                // keys' or values' bytes of a tile
+    static constexpr int HALF = KP_KEYS * 128;             // float16 values of a tile, 64 columns
+    static constexpr int V16 = HALF * (D / 64);
+    static constexpr int Q = 0, K = 2 * Q_BYTES, V = K + KP_STAGES * RAW, H = V + KP_STAGES * RAW;
+    static constexpr int SCALES = H + KP_STAGES * V16;     // [stage][group] (key's, value's)
+    static constexpr int FACTOR = SCALES + KP_STAGES * KP_GROUPS * 8;
+    static constexpr int BARS = FACTOR + KP_ROWS * 4;
+    static constexpr int BYTES = BARS + (3 * KP_STAGES + 7) * 8 + 16;
+    static constexpr int SHARE_LD = D + 4;
+    static_assert(K % 1024 == 0 && V % 1024 == 0 && H % 1024 == 0 && SCALES % 8 == 0, "swizzled tiles");
+    static_assert(KP_ROWS * (SHARE_LD + 2) * 4 <= SCALES - K, "a share of the keys lies where the tiles were");
+};
 
 // D += A B with A (float16, two to a 32-bit column) in tensor memory
 __device__ __forceinline__ void umma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -59,15 +65,18 @@ __device__ __forceinline__ void umma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, ui
         : "memory");
 }
 
-__global__ void __launch_bounds__(KP_THREADS, 2)
+template <int D>
+__global__ void __launch_bounds__(KP_THREADS, D == 64 ? 2 : 1)
 attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* out, const __grid_constant__ CUtensorMap map, const K8Args a) {
+    using L = KpSmem<D>;
+    constexpr uint32_t COLS = D == 64 ? 256 : 512;         // tensor memory: two of 64 columns for scores, two of D for outputs
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map)) : "memory");
     pdl_wait();
     const uint32_t base = smem_u32(smem_raw);
-    const uint32_t bars = base + KP_BARS;
+    const uint32_t bars = base + L::BARS;
     auto kv_full = [&](int s) { return bars + (uint32_t)s * 8; };
     auto v_full = [&](int s) { return bars + (uint32_t)(KP_STAGES + s) * 8; };
     auto kv_empty = [&](int s) { return bars + (uint32_t)(2 * KP_STAGES + s) * 8; };
@@ -75,9 +84,9 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
     auto p_full = [&](int b) { return bars + (uint32_t)(3 * KP_STAGES + 2 + b) * 8; };
     auto pv_full = [&](int b) { return bars + (uint32_t)(3 * KP_STAGES + 4 + b) * 8; };
     const uint32_t q_full = bars + (3 * KP_STAGES + 6) * 8, tmem_slot = q_full + 8;
-    float* row_factor = reinterpret_cast<float*>(smem_raw + KP_FACTOR);
-    float* share_o = reinterpret_cast<float*>(smem_raw + KP_K);
-    float2* share_ml = reinterpret_cast<float2*>(share_o + KP_ROWS * KP_SHARE_LD);
+    float* row_factor = reinterpret_cast<float*>(smem_raw + L::FACTOR);
+    float* share_o = reinterpret_cast<float*>(smem_raw + L::K);
+    float2* share_ml = reinterpret_cast<float2*>(share_o + KP_ROWS * L::SHARE_LD);
 
     const int max_split = a.nsplit, Hkv = a.Hkv, H = a.H, P = a.P, G = H / Hkv;
     // the KV head fastest and the tiles in reverse: a causal tile late in its sequence reads the most keys, so the longest CTAs start first
@@ -114,7 +123,7 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 3) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(256u) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -124,8 +133,9 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
     const uint32_t tmem_pv = tmem + 2 * KP_KEYS;         // outputs at columns 128 + 64 b; S_b at [64 b, 64 b + 64)
 
     // the first four warps give registers up and the softmax warps (a whole row of scores each) take them: 128 x 48 + 256 x 96 of 384 x 80
+    // (heads of 128: one CTA an SM has registers for all)
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if constexpr (D == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         if (warp == 0) {
             // lane i knows the page and the scales of 16 positions of one of eight tiles, and brings the page (or 64 positions of it) if they are its
             // first of the tile; asked for 16 and 8 tiles ahead
@@ -141,7 +151,7 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
             };
             int page = -1, page_next = page_of(0), page_after = page_of(1);
             float2 scale = make_float2(1.f, 1.f), scale_next = scales_of(page_next);
-            float2* sc = reinterpret_cast<float2*>(smem_raw + KP_SCALES);
+            float2* sc = reinterpret_cast<float2*>(smem_raw + L::SCALES);
             for (int it = 0; it < n_tiles; ++it) {
                 const int s = it % KP_STAGES;
                 if ((it & 7) == 0) {
@@ -157,37 +167,38 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
                 const int loads = __popc(__ballot_sync(0xffffffffu, mine));
                 if (mine) {
                     const int row = (page * 2 * Hkv + kvh) * P + ((tile_j0(it) + group * 16) & (P - 1));
-                    const uint32_t at = base + (uint32_t)(s * KP_RAW + group * 16 * KP_D);
-                    tma_load_2d(at + KP_K, &map, 0, row, kv_full(s));
-                    tma_load_2d(at + KP_V, &map, 0, row + Hkv * P, kv_full(s));
+                    const uint32_t at = base + (uint32_t)(s * L::RAW + group * 16 * D);
+                    tma_load_2d(at + L::K, &map, 0, row, kv_full(s));
+                    tma_load_2d(at + L::V, &map, 0, row + Hkv * P, kv_full(s));
                 }
                 if (ours) sc[s * KP_GROUPS + group] = scale;
                 __syncwarp();
                 // (the phase ends with this arrival and the bytes, whichever come last)
-                if (lane == 0) mbar_expect_tx(kv_full(s), (uint32_t)(loads * 2 * per * KP_D));
+                if (lane == 0) mbar_expect_tx(kv_full(s), (uint32_t)(loads * 2 * per * D));
             }
         } else if (warp < 3) {
-            // ---- V in float16: a thread turns four chunks of 16 bytes a tile ----
+            // ---- V in float16, 64 columns a tile: a thread turns four or eight chunks of 16 bytes ----
             const int t = tid - 32;
             bool ok = true;
             for (int it = 0; it < n_tiles; ++it) {
                 const int s = it % KP_STAGES, j0 = tile_j0(it);
                 ok = k8_wait(kv_full(s), (uint32_t)((it / KP_STAGES) & 1));
                 if (!__all_sync(0xffffffffu, ok)) break;
-                const unsigned char* raw = smem_raw + KP_V + s * KP_RAW;
-                unsigned char* wide = smem_raw + KP_H + s * KP_V16;
+                const unsigned char* raw = smem_raw + L::V + s * L::RAW;
+                unsigned char* wide = smem_raw + L::H + s * L::V16;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = (t >> 2) + 16 * i, chunk = t & 3, j = j0 + key;
-                    uint4 v = *reinterpret_cast<const uint4*>(raw + swizzled<KP_D>(key, chunk));
+                for (int i = 0; i < D / 16; ++i) {
+                    const int at = t + 64 * i, key = at / (D / 16), chunk = at % (D / 16), j = j0 + key;
+                    uint4 v = *reinterpret_cast<const uint4*>(raw + swizzled<D>(key, chunk));
                     if (j < lo || j > pos_last) v = make_uint4(0u, 0u, 0u, 0u);
                     uint4 x, y;
                     x.x = e4m3x2_to_half2((uint16_t)v.x), x.y = e4m3x2_to_half2((uint16_t)(v.x >> 16));
                     x.z = e4m3x2_to_half2((uint16_t)v.y), x.w = e4m3x2_to_half2((uint16_t)(v.y >> 16));
                     y.x = e4m3x2_to_half2((uint16_t)v.z), y.y = e4m3x2_to_half2((uint16_t)(v.z >> 16));
                     y.z = e4m3x2_to_half2((uint16_t)v.w), y.w = e4m3x2_to_half2((uint16_t)(v.w >> 16));
-                    *reinterpret_cast<uint4*>(wide + swizzled<128>(key, 2 * chunk)) = x;
-                    *reinterpret_cast<uint4*>(wide + swizzled<128>(key, 2 * chunk + 1)) = y;
+                    unsigned char* to = wide + (chunk >> 2) * L::HALF;
+                    *reinterpret_cast<uint4*>(to + swizzled<128>(key, 2 * (chunk & 3))) = x;
+                    *reinterpret_cast<uint4*>(to + swizzled<128>(key, 2 * (chunk & 3) + 1)) = y;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -196,8 +207,8 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
         } else {
             // ---- the products: the warp walks the tiles together, one elected lane issues ----
             constexpr uint32_t id_s = idesc8(KP_ROWS, KP_KEYS, false);
-            constexpr uint32_t id_pv = (1u << 4) | (1u << 16) | ((uint32_t)(KP_D >> 3) << 17) | ((uint32_t)(KP_ROWS >> 4) << 24);   // f16, V [key][d]: MN-major
-            const uint64_t qd = desc8<KP_D>(base + KP_Q);
+            constexpr uint32_t id_pv = (1u << 4) | (1u << 16) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(KP_ROWS >> 4) << 24);   // f16, 64 columns, V [key][d]: MN-major
+            const uint64_t qd = desc8<D>(base + L::Q);
             auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, k8_wait(bar, parity)) != 0; };
             bool ok = n_tiles > 0 && wait(q_full, 0);
             auto issue_s = [&](int j) {
@@ -205,13 +216,13 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
                 ok = ok && wait(kv_full(s), (uint32_t)((j / KP_STAGES) & 1));
                 if (!ok) return;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint64_t kd = desc8<KP_D>(base + KP_K + (uint32_t)s * KP_RAW);
+                const uint64_t kd = desc8<D>(base + L::K + (uint32_t)s * L::RAW);
                 if (elect_lane()) {
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
-                        for (int k = 0; k < KP_D / 32; ++k)
-                            umma_f8(tmem + (uint32_t)b * KP_KEYS, qd + (uint64_t)(t * KP_Q_BYTES / 16 + 2 * k), kd + 2 * k, id_s, t + k > 0 ? 1u : 0u);
+                        for (int k = 0; k < D / 32; ++k)
+                            umma_f8(tmem + (uint32_t)b * KP_KEYS, qd + (uint64_t)(t * L::Q_BYTES / 16 + 2 * k), kd + 2 * k, id_s, t + k > 0 ? 1u : 0u);
                     umma_commit(s_full(b));
                 }
                 __syncwarp();
@@ -223,11 +234,14 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
                 ok = wait(p_full(b), (uint32_t)((j >> 1) & 1)) && wait(v_full(s), (uint32_t)((j / KP_STAGES) & 1));
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint64_t vd = desc8<128>(base + KP_H + (uint32_t)s * KP_V16);
+                const uint64_t vd = desc8<128>(base + L::H + (uint32_t)s * L::V16);
                 if (elect_lane()) {
 #pragma unroll
-                    for (int k = 0; k < KP_KEYS / 16; ++k)           // 16 keys: 8 columns of P, 16 rows of V
-                        umma_f16_ta(tmem_pv + (uint32_t)b * KP_D, tmem + (uint32_t)(b * KP_KEYS + 8 * k), vd + 128 * k, id_pv, (j > 1 || k > 0) ? 1u : 0u);
+                    for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+                        for (int k = 0; k < KP_KEYS / 16; ++k)       // 16 keys: 8 columns of P, 16 rows of V
+                            umma_f16_ta(tmem_pv + (uint32_t)(b * D + 64 * h), tmem + (uint32_t)(b * KP_KEYS + 8 * k), vd + (uint64_t)(h * L::HALF / 16 + 128 * k),
+                                        id_pv, (j > 1 || k > 0) ? 1u : 0u);
                 }
                 __syncwarp();
                 // (in order behind the product that reads P_j, where S_{j+2} goes; the group's next wait is for it, and for that product)
@@ -242,30 +256,29 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
         }
         __syncwarp();
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
+        if constexpr (D == 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
         const int g_shift = __ffs(G) - 1;
         {
             // ---- q's terms: a row two threads (rows past the tile are zero) ----
-            const int rr = (tid - 128) >> 1, c0 = (tid & 1) * 32;
-            float x[32], big = 0.f;
+            const int rr = (tid - 128) >> 1, c0 = (tid & 1) * (D / 2);
+            uint4 raw[D / 16];
+            float big = 0.f;
             bool fine = true;
-            const __nv_bfloat16* src = q + ((size_t)(tok0 + (rr >> g_shift)) * H + kvh * G + (rr & (G - 1))) * KP_D + c0;
+            const __nv_bfloat16* src = q + ((size_t)(tok0 + (rr >> g_shift)) * H + kvh * G + (rr & (G - 1))) * D + c0;
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-                uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-                if (rr < rows) raw = *reinterpret_cast<const uint4*>(src + e);
-                const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+            for (int e = 0; e < D / 16; ++e) {
+                raw[e] = make_uint4(0u, 0u, 0u, 0u);
+                if (rr < rows) raw[e] = *reinterpret_cast<const uint4*>(src + 8 * e);
+            }
+#pragma unroll
+            for (int e = 0; e < D / 16; ++e)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    x[e + 2 * k] = __uint_as_float(w[k] << 16);
-                    x[e + 2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+                    const uint32_t w = (&raw[e].x)[k];
+                    const float u = fabsf(__uint_as_float(w << 16)), v = fabsf(__uint_as_float(w & 0xffff0000u));
+                    big = fmaxf(big, fmaxf(u, v));
+                    fine = fine && u <= 3.4e38f && v <= 3.4e38f;
                 }
-            }
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-                big = fmaxf(big, fabsf(x[e]));
-                fine = fine && fabsf(x[e]) <= 3.4e38f;
-            }
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
             fine = __shfl_xor_sync(0xffffffffu, (int)fine, 1) != 0 && fine;
             int e2 = (__float_as_int(big) >> 23) - 127;
@@ -273,23 +286,24 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
             const float up = exp2i(7 - e2);
             if ((tid & 1) == 0) row_factor[rr] = fine ? a.scale * K8_LOG2E * exp2i(e2 - 7) : NAN;        // (no score of a row that is not finite is)
 #pragma unroll
-            for (int e = 0; e < 32; e += 16) {
+            for (int e = 0; e < D / 2; e += 16) {
                 uint32_t t1[4], t2[4];
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     t1[w] = t2[w] = 0;
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        const float u = x[e + 4 * w + 2 * k] * up, v = x[e + 4 * w + 2 * k + 1] * up;
+                        const uint32_t two = (&raw[(e + 4 * w) >> 3].x)[((e + 4 * w) & 7) / 2 + k];
+                        const float u = __uint_as_float(two << 16) * up, v = __uint_as_float(two & 0xffff0000u) * up;
                         const uint16_t first = to_e4m3x2(u, v);
                         const float2 back = half2_floats(e4m3x2_to_half2(first));
                         t1[w] |= (uint32_t)first << (16 * k);
                         t2[w] |= (uint32_t)to_e4m3x2(u - back.x, v - back.y) << (16 * k);
                     }
                 }
-                unsigned char* at = smem_raw + KP_Q + swizzled<KP_D>(rr, (c0 + e) >> 4);
+                unsigned char* at = smem_raw + L::Q + swizzled<D>(rr, (c0 + e) >> 4);
                 *reinterpret_cast<uint4*>(at) = make_uint4(t1[0], t1[1], t1[2], t1[3]);
-                *reinterpret_cast<uint4*>(at + KP_Q_BYTES) = make_uint4(t2[0], t2[1], t2[2], t2[3]);
+                *reinterpret_cast<uint4*>(at + L::Q_BYTES) = make_uint4(t2[0], t2[1], t2[2], t2[3]);
             }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -299,7 +313,7 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
         // ---- the weights ----
         const int grp = (warp - 4) >> 2, r = (tid - 128) & 127, quarter = warp & 3;
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-        const uint32_t out_addr = tmem_pv + (uint32_t)grp * KP_D + lane_base;
+        const uint32_t out_addr = tmem_pv + (uint32_t)grp * D + lane_base;
         const int pos_r = r < rows ? pos_first + (r >> g_shift) : -1;
         const int lo_r = first_seen(pos_r, a.window), lo_last = first_seen(pos_last, a.window);
         const float c_row = row_factor[r];
@@ -315,7 +329,7 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
             float x[2][32];                              // the row's 64 products stay in registers
             tmem_ld32(s_addr, x[0]);
             tmem_ld32(s_addr + 32u, x[1]);
-            const float2* sc = reinterpret_cast<const float2*>(smem_raw + KP_SCALES) + s * KP_GROUPS;
+            const float2* sc = reinterpret_cast<const float2*>(smem_raw + L::SCALES) + s * KP_GROUPS;
             float kc[KP_GROUPS], ev[KP_GROUPS], inv_v[KP_GROUPS];
 #pragma unroll
             for (int g = 0; g < KP_GROUPS; ++g) {
@@ -352,7 +366,7 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
                     // (the product of the group's tile before has landed: it was issued ahead of these scores, whose commit covers both)
                     const float f = m_new == -INFINITY ? 1.0f : k8_exp2(m_ref - m_new);
 #pragma unroll
-                    for (int c = 0; c < KP_D; c += 16) {          // (narrow: the scores stay in registers)
+                    for (int c = 0; c < D; c += 16) {          // (narrow: the scores stay in registers)
                         float part[16];
                         tmem_ld16(out_addr + (uint32_t)c, part);
 #pragma unroll
@@ -399,7 +413,7 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
         ok = __all_sync(0xffffffffu, ok);
         // the second group's maximum and sum of each row go to q's first term, which no product reads any more: the last S of either group was issued
         // before the P V waited for above
-        float2* other = reinterpret_cast<float2*>(smem_raw + KP_Q) + r;
+        float2* other = reinterpret_cast<float2*>(smem_raw + L::Q) + r;
         if (grp == 1 && n_tiles > 1) *other = make_float2(m_ref, l_row);
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         asm volatile("bar.sync 5, 256;" ::: "memory");
@@ -413,7 +427,7 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
             l_row = two ? fmaf(l_row, f0, theirs.y * f1) : l_row;
             m_ref = m_all;
             const int tok = tok0 + (r >> g_shift), head = kvh * G + (r & (G - 1));
-            __nv_bfloat16* dst = out + ((size_t)tok * H + head) * KP_D;
+            __nv_bfloat16* dst = out + ((size_t)tok * H + head) * D;
             float inv = 1.f, gate = 1.f;
             if (nsplit == 1) {
                 if (a.sink && m_ref > -INFINITY) l_row += k8_exp2(KP_LIFT - m_ref);
@@ -421,16 +435,16 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
                 if (r < rows) gate = k8_gate<__nv_bfloat16>(a, tok, head);
             }
 #pragma unroll
-            for (int c = 0; c < KP_D; c += 16) {
+            for (int c = 0; c < D; c += 16) {
                 float v[16], more[16];
                 tmem_ld16(out_addr + (uint32_t)c, v);
-                if (two) tmem_ld16(out_addr + (uint32_t)(KP_D + c), more);
+                if (two) tmem_ld16(out_addr + (uint32_t)(D + c), more);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) v[e] = two ? fmaf(v[e], f0, more[e] * f1) : v[e];
                 if (nsplit > 1) {
 #pragma unroll
                     for (int e = 0; e < 16; e += 4)
-                        *reinterpret_cast<float4*>(share_o + r * KP_SHARE_LD + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                        *reinterpret_cast<float4*>(share_o + r * L::SHARE_LD + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
                 } else if (r < rows) {
                     uint32_t packed[8];
 #pragma unroll
@@ -455,14 +469,14 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
             const int tok = tok0 + r / G, head = kvh * G + r % G;
             auto merge = [&](auto shares) {
                 // eight reads of four columns a thread, whatever the number of shares, all in flight together
-                constexpr int NS = decltype(shares)::value, PER = KP_D / 2 / NS;
+                constexpr int NS = decltype(shares)::value, PER = D / 2 / NS;
                 const int c0 = split * 2 * PER + ((tid - 128) >> 7) * PER;
                 float2 ml[NS];
                 float4 o[NS][PER / 4];
 #pragma unroll
                 for (int sp = 0; sp < NS; ++sp) {
                     ml[sp] = cluster.map_shared_rank(share_ml, sp)[r];
-                    const float* from = cluster.map_shared_rank(share_o, sp) + r * KP_SHARE_LD + c0;
+                    const float* from = cluster.map_shared_rank(share_o, sp) + r * L::SHARE_LD + c0;
 #pragma unroll
                     for (int k = 0; k < PER / 4; ++k) o[sp][k] = *reinterpret_cast<const float4*>(from + 4 * k);
                 }
@@ -487,7 +501,7 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
                         for (int e = 0; e < 4; ++e) v[e] = fmaf((&o[sp][k].x)[e], ml[sp].x, v[e]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] = k8_apply<__nv_bfloat16>(v[e] * inv, a, gate);
-                    Quad<__nv_bfloat16>::store(out + ((size_t)tok * H + head) * KP_D + c0 + 4 * k, make_float4(v[0], v[1], v[2], v[3]));
+                    Quad<__nv_bfloat16>::store(out + ((size_t)tok * H + head) * D + c0 + 4 * k, make_float4(v[0], v[1], v[2], v[3]));
                 }
             };
             if (nsplit == 2) merge(std::integral_constant<int, 2>());
@@ -501,30 +515,34 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
     __syncthreads();
     if (warp == 3) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS) : "memory");
     }
+}
+
+template <int D>
+cudaError_t kp_launch(const void* q, const float* scales, void* out, const CUtensorMap& map, const K8Args& a, cudaStream_t stream) {
+    const cudaError_t e = cudaFuncSetAttribute(attn_kv8_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, KpSmem<D>::BYTES);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.items * a.Hkv * a.nsplit));
+    cfg.blockDim = dim3(KP_THREADS);
+    cfg.dynamicSmemBytes = KpSmem<D>::BYTES;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    cfg.attrs = attr;
+    cfg.numAttrs = k8_attributes(attr, a.nsplit);
+    return cudaLaunchKernelEx(&cfg, attn_kv8_prefill_kernel<D>, (const __nv_bfloat16*)q, scales, (__nv_bfloat16*)out, map, a);
 }
 
 }  // namespace
 
-// The arguments of tk_attn_kv8 for tiles (attention_kv8.cu checks them): bfloat16, heads of 64, a group of query heads that divides 128, pages that are a power
-// of two and 16 or more.
-int tk_attn_kv8_prefill_tc(const void* q, const void* pool, const float* scales, void* out, const void* args, cudaStream_t stream) {
+// The arguments of tk_attn_kv8 for tiles (attention_kv8.cu checks them): bfloat16, a group of query heads that divides 128, pages that are a power of two
+// and 16 or more.
+int tk_attn_kv8_prefill_tc(const void* q, const void* pool, const float* scales, void* out, const void* args, int D, cudaStream_t stream) {
     const K8Args& a = *static_cast<const K8Args*>(args);
     CUtensorMap map = {};
-    TK_CHECK_ARG(k8_map(&map, pool, KP_D, a.P < KP_KEYS ? a.P : KP_KEYS), "attn_kv8: cuTensorMapEncodeTiled failed");
-    cudaError_t e = cudaFuncSetAttribute(attn_kv8_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, KP_SMEM);
-    if (e == cudaSuccess) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)(a.items * a.Hkv * a.nsplit));
-        cfg.blockDim = dim3(KP_THREADS);
-        cfg.dynamicSmemBytes = KP_SMEM;
-        cfg.stream = stream;
-        cudaLaunchAttribute attr[2];
-        cfg.attrs = attr;
-        cfg.numAttrs = k8_attributes(attr, a.nsplit);
-        e = cudaLaunchKernelEx(&cfg, attn_kv8_prefill_kernel, (const __nv_bfloat16*)q, scales, (__nv_bfloat16*)out, map, a);
-    }
+    TK_CHECK_ARG(k8_map(&map, pool, D, a.P < KP_KEYS ? a.P : KP_KEYS), "attn_kv8: cuTensorMapEncodeTiled failed");
+    const cudaError_t e = D == 64 ? kp_launch<64>(q, scales, out, map, a, stream) : kp_launch<128>(q, scales, out, map, a, stream);
     if (e != cudaSuccess) {
         tk_set_error("attn_kv8: launch failed: %s", cudaGetErrorString(e));
         cudaGetLastError();

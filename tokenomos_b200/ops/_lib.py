@@ -136,7 +136,7 @@ _SIGNATURES = {
     "tk_attn_kv8_supported": [I, I, I],
     "tk_attn_kv8_tokens": [I, I, I, I, I],
     "tk_attn_kv8_prefill_supported": [I, I, I, I, I],
-    "tk_attn_kv8_prefill_splits": [I, I, I, I, I, I],
+    "tk_attn_kv8_prefill_splits": [I, I, I, I, I, I, I],
     "tk_attn_kv8_status": [],
     "tk_attn_kv8_splits": [I, I, I, I, I, I, I, I],
     "tk_attn_kv8_single_tc": [I, I],

@@ -173,7 +173,7 @@ def attention_kv8_prefill(q: torch.Tensor, pool: torch.Tensor, scales: torch.Ten
         reach = min(int(longest), abs(int(window)) + T) if window else int(longest)
         rows = 0
         if _lib.call("tk_attn_kv8_prefill_supported", H, Hkv, D, P, code):
-            nsplit = _lib.call("tk_attn_kv8_prefill_splits", T, n, H, Hkv, reach, _sms(q.get_device()))
+            nsplit = _lib.call("tk_attn_kv8_prefill_splits", T, n, H, Hkv, D, reach, _sms(q.get_device()))
         else:
             rows = _lib.call("tk_attn_kv8_tokens", H, Hkv, D, P, code) * (H // Hkv)
             nsplit = _lib.call("tk_attn_kv8_splits", n, H, Hkv, D, reach, reach, _sms(q.get_device()), 0)
