@@ -676,13 +676,13 @@ def test_entry_points_refuse_shapes_that_are_not_built():
     for H, G, D in ((4, 3, 64), (17, 1, 64), (4, 2, 96), (4, 0, 64)):
         assert not ops.kv8_supported(H, G, D)
         with pytest.raises(KernelError, match="not taken"):
-            _lib.call("tk_attn_kv8", 256, 256, 256, 256, 256, 256, 256, 1, None, None, 1, H, G, D, 16, 0, 1.0, 1, None, None, 0, 0, 1, None)
+            _lib.call("tk_attn_kv8", 256, 256, 256, 256, 256, 256, 256, 1, None, None, 1, H, G, D, 16, 0, 1.0, 1, 99, 1, None, None, 0, 0, 1, None)
     with pytest.raises(KernelError, match="positive"):
-        _lib.call("tk_attn_kv8", 256, 256, 256, 256, 256, 256, 256, 1, None, None, 1, 4, 2, 64, 16, 0, 0.0, 1, None, None, 0, 0, 1, None)
+        _lib.call("tk_attn_kv8", 256, 256, 256, 256, 256, 256, 256, 1, None, None, 1, 4, 2, 64, 16, 0, 0.0, 1, 99, 1, None, None, 0, 0, 1, None)
     with pytest.raises(KernelError, match="bad sizes"):
-        _lib.call("tk_attn_kv8", 256, 256, 256, 256, 256, 256, 256, 1, None, None, 1, 4, 2, 64, 16, 0, 1.0, 4, None, None, 0, 0, 0, None)
+        _lib.call("tk_attn_kv8", 256, 256, 256, 256, 256, 256, 256, 1, None, None, 1, 4, 2, 64, 16, 0, 1.0, 4, 99, 1, None, None, 0, 0, 0, None)
     with pytest.raises(KernelError, match="at most 16"):
-        _lib.call("tk_attn_kv8", 256, 256, 256, 256, 256, 256, 256, 1, None, None, 1, 4, 2, 64, 16, 0, 1.0, 17, None, None, 0, 0, 1, None)
+        _lib.call("tk_attn_kv8", 256, 256, 256, 256, 256, 256, 256, 1, None, None, 1, 4, 2, 64, 16, 0, 1.0, 17, 99, 1, None, None, 0, 0, 1, None)
 
 
 def test_tensors_of_the_host_are_refused():

@@ -416,7 +416,8 @@ cudaError_t k8_launch(const void* q, const void* pool, const float* scales, void
     constexpr int ring = PAGE16 ? K8_WARPS * K8_DEPTH * (4096 + 8) : 0;
     constexpr int smem = ring > shares ? ring : shares;
     if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(attn_kv8_kernel<T, D, PAGE16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        static std::atomic<uint64_t> done{0};
+        const cudaError_t e = k8_allow(attn_kv8_kernel<T, D, PAGE16>, smem, false, done);
         if (e != cudaSuccess) return e;
     }
     return tk_launch(attn_kv8_kernel<T, D, PAGE16>, dim3((unsigned)(a.items * a.Hkv * a.nsplit)), dim3(K8_THREADS), smem, stream, (const T*)q,
@@ -505,23 +506,33 @@ TK_API int tk_attn_kv8_status() {
     return 0;
 }
 
-// q, out: [T, H, D]; pool: [pages, 2, Hkv, P, D] bytes, scales: [pages, 2, Hkv]. item_tok0 / item_ntok: tiles of at most tk_attn_kv8_tokens tokens of one
+// tokens: rows of q. q, out: [T, H, D]; pool: [pages, 2, Hkv, P, D] bytes, scales: [pages, 2, Hkv]. item_tok0 / item_ntok: tiles of at most tk_attn_kv8_tokens tokens of one
 // sequence at consecutive positions (0 tokens: skipped); item_ntok null: single tokens' rows (negative: skipped; item_tok0 null too: rows 0, 1, ...).
-// window: see first_seen. scratch: items * H * (tokens a tile, or 1) * nsplit * (D + 4) floats when nsplit > 1. gate: [T, >= H], the per-head output gate.
+// nsplit 0: chosen here, for sequences of at most `longest` positions (the tcgen05 kernels, which need no scratch). window: see first_seen. scratch: items * H * (tokens a tile, or 1) * nsplit * (D + 4) floats when nsplit > 1. gate: [T, >= H], the per-head output gate.
 TK_API int tk_attn_kv8(const void* q, const void* pool, const float* scales, void* out, const int* positions, const int* tok_seq,
                        const int* block_table, int bt_stride, const int* item_tok0, const int* item_ntok, int items, int H, int Hkv, int D,
-                       int P, int window, float scale, int nsplit, float* scratch, const void* gate, int64_t ldg, int sink, int dtype,
-                       cudaStream_t stream) {
+                       int P, int window, float scale, int nsplit, int longest, int tokens, float* scratch, const void* gate, int64_t ldg, int sink,
+                       int dtype, cudaStream_t stream) {
     TK_CHECK_ARG(tk_attn_kv8_supported(H, Hkv, D), "attn_kv8: shape H=%d Hkv=%d D=%d is not taken (heads of 64 or 128, up to %d a KV head)", H,
                  Hkv, D, K8_ROWS);
     const bool meets_in_scratch = item_ntok == nullptr ? !tk_attn_kv8_single_tc(P, dtype) : !tk_attn_kv8_prefill_supported(H, Hkv, D, P, dtype);
-    TK_CHECK_ARG(items >= 0 && P > 0 && nsplit >= 1 && (nsplit == 1 || scratch != nullptr || !meets_in_scratch), "attn_kv8: bad sizes");
+    TK_CHECK_ARG(items >= 0 && P > 0 && nsplit >= (meets_in_scratch ? 1 : 0) && (nsplit <= 1 || scratch != nullptr || !meets_in_scratch), "attn_kv8: bad sizes");
     TK_CHECK_ARG(item_ntok == nullptr || item_tok0 != nullptr, "attn_kv8: tiles have first tokens");
     TK_CHECK_ARG((int64_t)items * Hkv * nsplit < 0x7fffffff, "attn_kv8: %d splits of %d items", nsplit, items);
     TK_CHECK_ARG(scale > 0.f, "attn_kv8: the scores' factor is positive");
     TK_CHECK_ARG(dtype == TK_F32 || dtype == TK_BF16, "attn_kv8: unknown dtype %d", dtype);
     TK_CHECK_ARG((uintptr_t)q % 16 == 0 && (uintptr_t)pool % 16 == 0 && (uintptr_t)out % 16 == 0, "attn_kv8: 16-byte aligned tensors");
     if (items == 0) return 0;
+    if (nsplit == 0) {
+        int device = 0, sms = 0;
+        if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+            tk_set_error("attn_kv8: no device");
+            return -1;
+        }
+        const int64_t reach = window == 0 ? longest : (int64_t)(window < 0 ? -window : window) + (item_ntok != nullptr ? tokens : 0);
+        const int most = (int)(reach < longest ? reach : longest);
+        nsplit = item_ntok != nullptr ? tk_attn_kv8_prefill_splits(tokens, items, H, Hkv, D, most, sms) : tk_attn_kv8_splits(items, H, Hkv, D, longest, most, sms, 1);
+    }
     int shift = -1;
     if ((P & (P - 1)) == 0)
         for (shift = 0; (1 << shift) < P;) ++shift;

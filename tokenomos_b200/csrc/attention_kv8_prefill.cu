@@ -521,7 +521,8 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
 
 template <int D>
 cudaError_t kp_launch(const void* q, const float* scales, void* out, const CUtensorMap& map, const K8Args& a, cudaStream_t stream) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_kv8_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, KpSmem<D>::BYTES);
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = k8_allow(attn_kv8_prefill_kernel<D>, KpSmem<D>::BYTES, false, done);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.items * a.Hkv * a.nsplit));

@@ -459,8 +459,8 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
 template <int D, int NR>
 cudaError_t k8t_launch(const void* q, const float* scales, void* out, const CUtensorMap& map, const K8Args& a, cudaStream_t stream) {
     constexpr int smem = K8tSmem<D, NR>::BYTES;
-    cudaError_t e = cudaFuncSetAttribute(attn_kv8_tc_kernel<D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess && a.nsplit > 8) e = cudaFuncSetAttribute(attn_kv8_tc_kernel<D, NR>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = k8_allow(attn_kv8_tc_kernel<D, NR>, smem, true, done);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.items * a.Hkv * a.nsplit));

@@ -2,6 +2,8 @@
 // a row's keys that several CTAs have seen.
 #pragma once
 
+#include <atomic>
+
 #include "kv8.cuh"
 
 namespace {
@@ -53,6 +55,18 @@ inline int k8_take_status() {
     if (cudaMemcpyFromSymbol(&v, g_k8_error, sizeof(int)) != cudaSuccess) return -1;
     if (v != 0) cudaMemcpyToSymbol(g_k8_error, &zero, sizeof(int));
     return v;
+}
+
+// Dynamic shared memory (and clusters of more than eight CTAs) that a kernel may have, asked for once a device: `done` holds a bit a device.
+template <typename K>
+inline cudaError_t k8_allow(K kernel, int smem, bool wide, std::atomic<uint64_t>& done) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess || (device < 64 && done.load(std::memory_order_relaxed) >> device & 1)) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && wide) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && device < 64) done.fetch_or(1ull << device, std::memory_order_relaxed);
+    return e;
 }
 
 struct K8Args {

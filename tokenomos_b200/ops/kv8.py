@@ -83,7 +83,7 @@ def qk_norm_rope_write8(qkv: torch.Tensor, pool: torch.Tensor, scales: torch.Ten
     _check_layout(name, T, positions, tok_seq, block_table)
     rot = 2 * inv_freq.numel()
     ops._f32vec(inv_freq, "inv_freq", rot // 2)
-    q = torch.empty(T, heads, head_dim, dtype=qkv.dtype, device=qkv.device)
+    q = qkv.new_empty((T, heads, head_dim))
     _lib.call("tk_qk_norm_rope_write8", qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1], q.data_ptr(), pool.data_ptr(),
               scales.data_ptr(), ops._ptr(ops._f32vec(wq, "q_norm weight", head_dim)), ops._ptr(ops._f32vec(wk, "k_norm weight", head_dim)),
               float(eps), inv_freq.data_ptr(), float(cs_mult), int(bool(interleaved)), positions.data_ptr(), tok_seq.data_ptr(),
@@ -117,16 +117,16 @@ def _sms(device: int) -> int:
     return n
 
 
-def _attend(q, pool, scales, out, positions, tok_seq, block_table, tok0, ntok, items, nsplit, rows, shape, window, scale, gate, sink):
-    """``rows`` > 0: the shares of a tile (of so many rows) meet in scratch memory."""
+def _attend(q, pool, scales, out, positions, tok_seq, block_table, tok0, ntok, items, nsplit, rows, shape, window, scale, longest, gate, sink):
+    """``nsplit`` 0: the entry point chooses; above 1 the shares of a tile of ``rows`` rows meet in scratch memory."""
     T, H, Hkv, P, D, code = shape
     scratch = None
-    if nsplit > 1 and rows:
+    if nsplit > 1:
         scratch = torch.empty(items * Hkv * nsplit * rows * (D + 4), dtype=torch.float32, device=q.device)
     _lib.call("tk_attn_kv8", q.data_ptr(), pool.data_ptr(), scales.data_ptr(), out.data_ptr(), positions.data_ptr(), tok_seq.data_ptr(),
               block_table.data_ptr(), block_table.stride(0), ops._ptr(tok0), ops._ptr(ntok), items, H, Hkv, D, P, int(window or 0),
-              float(scale), nsplit, ops._ptr(scratch), ops._ptr(gate), gate.stride(0) if gate is not None else 0, int(bool(sink)), code,
-              ops._stream())
+              float(scale), nsplit, int(longest), T, ops._ptr(scratch), ops._ptr(gate), gate.stride(0) if gate is not None else 0,
+              1 if sink else 0, code, ops._stream())
 
 
 def _whole_pages(P: int) -> bool:
@@ -147,9 +147,11 @@ def attention_kv8_decode(q: torch.Tensor, pool: torch.Tensor, scales: torch.Tens
     n = shape[0] if tok_index is None else ops._i32(tok_index, "tok_index").numel()
     if n:
         T, H, Hkv, P, D, code = shape
-        tc = code == BF16 and _whole_pages(P)
-        nsplit = _lib.call("tk_attn_kv8_splits", n, H, Hkv, D, int(longest), abs(int(window)) if window else int(longest), _sms(q.get_device()), tc)
-        _attend(q, pool, scales, out, positions, tok_seq, block_table, tok_index, None, n, nsplit, 0 if tc else H // Hkv, shape, window, scale,
+        nsplit = 0
+        if code != BF16 or not _whole_pages(P):
+            nsplit = _lib.call("tk_attn_kv8_splits", n, H, Hkv, D, int(longest), abs(int(window)) if window else int(longest),
+                               _sms(q.get_device()), 0)
+        _attend(q, pool, scales, out, positions, tok_seq, block_table, tok_index, None, n, nsplit, H // Hkv, shape, window, scale, longest,
                 gate, sink)
 
 
@@ -170,14 +172,13 @@ def attention_kv8_prefill(q: torch.Tensor, pool: torch.Tensor, scales: torch.Ten
     if ops._i32(tile_ntok, "tile_ntok").numel() != n:
         raise KernelError(f"{name}: {n} first tokens for {tile_ntok.numel()} tiles")
     if n:
-        reach = min(int(longest), abs(int(window)) + T) if window else int(longest)
-        rows = 0
-        if _lib.call("tk_attn_kv8_prefill_supported", H, Hkv, D, P, code):
-            nsplit = _lib.call("tk_attn_kv8_prefill_splits", T, n, H, Hkv, D, reach, _sms(q.get_device()))
-        else:
+        nsplit = rows = 0
+        if code != BF16 or not _whole_pages(P) or not _lib.call("tk_attn_kv8_prefill_supported", H, Hkv, D, P, code):
+            reach = min(int(longest), abs(int(window)) + T) if window else int(longest)
             rows = _lib.call("tk_attn_kv8_tokens", H, Hkv, D, P, code) * (H // Hkv)
             nsplit = _lib.call("tk_attn_kv8_splits", n, H, Hkv, D, reach, reach, _sms(q.get_device()), 0)
-        _attend(q, pool, scales, out, positions, tok_seq, block_table, tile_tok0, tile_ntok, n, nsplit, rows, shape, window, scale, gate, sink)
+        _attend(q, pool, scales, out, positions, tok_seq, block_table, tile_tok0, tile_ntok, n, nsplit, rows, shape, window, scale, longest,
+                gate, sink)
 
 
 def attention_kv8_status() -> int:
