@@ -471,15 +471,20 @@ TK_API int tk_attn_kv8_prefill_splits(int tokens, int items, int H, int Hkv, int
 // CTA more and the launch runs in two waves), in clusters of at most eight with two tiles of 128 keys each, or of 16 with four (us by shares, 8 KV heads of 64:
 // a token behind 2,048 positions 14.9 unshared, 8.7 by 4, 7.6 by 8, 8.5 by 16; behind 30,000 136, 40, 24.7, 20.8; 8 tokens behind 32,000 49.0 by 6, 45.7 by 8, 61.7
 // by 10; 16 behind 4,000 15.3 by 4, 20.3 by 5; 64 behind up to 3,000 33.1 unshared, 38.9 by 2).
-// The mma.sync kernel's shares meet in scratch memory: enough to put four CTAs on every SM, of 256 keys at least.
+// The mma.sync kernel's shares meet in scratch memory and cost a second launch: none up to 512 keys, then 256 keys each at least, and as many as keep every CTA
+// resident (three an SM, heads of 128 two); where two would not, but a quarter of the places is free, three of long contexts all the same (us, 32-bit,
+// 8 KV heads of 64 with two query heads each: 2 prompts of up to 301 tokens 15.5 unshared, 24.0 by 2; 60 tokens behind 200 6.4 and 9.0; 256 behind 4,000 59.3, 52.1 by
+// 2, 48.7 by 3; 8 single tokens behind 4,000 34.5, 19.6 by 4, 16.8 by 6, 19.7 by 8; 64 behind 1,000 23.6, 26.8 by 2).
 TK_API int tk_attn_kv8_splits(int items, int H, int Hkv, int D, int longest, int reach, int sm_count, int tc) {
     const int64_t ctas = (int64_t)items * Hkv;
     if (ctas <= 0) return 1;
     const int64_t keys = longest < reach ? longest : reach;
     if (!tc) {
-        const int64_t fill = (4 * (int64_t)sm_count + ctas - 1) / ctas, by_keys = (keys + 255) / 256;
-        const int64_t n = fill < by_keys ? fill : by_keys;
-        return (int)(n < 1 ? 1 : n > 128 ? 128 : n);
+        const int64_t places = (int64_t)sm_count * (D == 64 ? 3 : 2);
+        int64_t n = places / ctas;
+        if (n == 1 && keys >= 2048 && 4 * ctas <= 3 * places) n = 3;
+        if (n > (keys + 255) / 256) n = (keys + 255) / 256;
+        return (int)(n < 1 || keys <= 512 ? 1 : n > 128 ? 128 : n);
     }
     const int64_t fit = (int64_t)sm_count * (D == 64 && H / Hkv <= 4 ? 4 : 2) / ctas, tiles = (keys + 127) / 128 + (reach < longest ? 1 : 0);
     if (fit >= 16 && tiles >= 64) return 16;
