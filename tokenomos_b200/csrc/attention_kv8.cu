@@ -7,7 +7,8 @@
 // keys; its warps walk groups of 32 (16 for heads of 128) keys in turn and are joined through shared memory, the CTAs of a
 // row through scratch memory and a second kernel.
 //
-// Bytes to operands without shared memory. The order of a product's inner index is free as long as both operands follow it, and the order of the output's columns is
+// Pages of 16 positions and more come by bulk copies, up to three units of 32 keys (heads of 128: 16) a warp in shared memory or on their way; smaller or odd ones are read by
+// each lane. From bytes to operands nothing is moved between lanes: the order of a product's inner index is free as long as both operands follow it, and the order of the output's columns is
 // too: a lane reads D / 4 bytes side by side of one key's row (16 bytes for D = 64; four lanes a row) and uses them as its fragments of all the D / 16
 // steps of q . k, with q's fragments laid out to match; and of a value row it reads D / 8 bytes, one for each of the D / 8 column tiles, so that two rows' bytes
 // interleave (prmt) into the pairs that a fragment holds. e4m3 is exact in float16.
@@ -23,7 +24,9 @@
 // Masked keys and values are never read (their bytes are zero in the products), so what an unwritten part of a page holds does not
 // matter. A row that sees no key is 0.
 //
-// Bound by HBM for long contexts; measured figures stand with the entry points.
+// Measured (32-bit, 16 heads over 8 of 64, one B200): two prompts of up to 301 tokens 15.5 us, 1,000 tokens 31.3, 8 single tokens behind 4,000 positions 16.9 (2.0 TB/s), one
+// behind 2,000 9.3. Bound by latency: 160 registers leave three CTAs an SM (the two prompts in two shares each 23.9 us, with two CTAs 27.3; units of 16 keys allow four: 12.9 for the two prompts, but 34.6 for the
+// 1,000 tokens and 49.5 for 34.5 unshared single tokens). A warp a row tile instead of a share of a CTA's keys was slower for prompts.
 #include <math.h>
 
 #include <type_traits>

@@ -19,6 +19,13 @@
 // by 8: weights stay below 2^15 of float16's 65,504, and reach down to 2^-31 of the row's largest); only then is the output read, scaled and
 // written back. At the end the first group merges both outputs, and up to eight CTAs (a cluster) that share a tile's keys merge theirs.
 //
+// Measured (32 heads over 8 of 64, one B200): a prompt of 2,048 tokens 41.6 us (the mma.sync kernel 124), 512 tokens behind 8,192 positions 71.1 (205), 512 behind
+// 30,000 224; heads of 128, 16 over 4: 1,000 tokens 18.4 (52), 256 behind 4,000 28.9 (75). Bound by each group's chain (scores, maximum, exponentials, weights
+// back, products), four groups an SM as tensor memory allows: exponentials' unit 49 % busy, ALU 42 %, tensor cores 24 %, 2.1 of 4 instructions a cycle.
+// Tried and slower: a warp a group for the products (71.1 became 79.6, 83.1 when those warps brought the tiles too: one warp keeps the groups out of step),
+// weights through shared memory so that the next scores need not wait for their product (86.8), the first half of a row's scores read twice instead of kept
+// (71.2, heads of 128 3 % slower), sums and products one by one instead of in pairs (74.0).
+//
 // Masking, sums, gate, sink and bounded waits are those of the other kernels of this cache; tk_attn_kv8_status() says where a wait gave up.
 #include <cooperative_groups.h>
 #include <math.h>
@@ -54,6 +61,13 @@ struct KpSmem {
     static_assert(K % 1024 == 0 && V % 1024 == 0 && H % 1024 == 0 && SCALES % 8 == 0, "swizzled tiles");
     static_assert(KP_ROWS * (SHARE_LD + 2) * 4 <= SCALES - K, "a share of the keys lies where the tiles were");
 };
+
+// the largest of three that are numbers
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 
 // D += A B with A (float16, two to a 32-bit column) in tensor memory
 __device__ __forceinline__ void umma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -210,28 +224,28 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
             constexpr uint32_t id_pv = (1u << 4) | (1u << 16) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(KP_ROWS >> 4) << 24);   // f16, 64 columns, V [key][d]: MN-major
             const uint64_t qd = desc8<D>(base + L::Q);
             auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, k8_wait(bar, parity)) != 0; };
+            auto keys_of = [&](int j) { return j >= n_tiles || wait(kv_full(j % KP_STAGES), (uint32_t)((j / KP_STAGES) & 1)); };
             bool ok = n_tiles > 0 && wait(q_full, 0);
-            auto issue_s = [&](int j) {
-                const int s = j % KP_STAGES, b = j & 1;
-                ok = ok && wait(kv_full(s), (uint32_t)((j / KP_STAGES) & 1));
-                if (!ok) return;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint64_t kd = desc8<D>(base + L::K + (uint32_t)s * L::RAW);
-                if (elect_lane()) {
+            auto issue_s = [&](int j) {                  // (one lane)
+                const int b = j & 1;
+                const uint64_t kd = desc8<D>(base + L::K + (uint32_t)(j % KP_STAGES) * L::RAW);
 #pragma unroll
-                    for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-                        for (int k = 0; k < D / 32; ++k)
-                            umma_f8(tmem + (uint32_t)b * KP_KEYS, qd + (uint64_t)(t * L::Q_BYTES / 16 + 2 * k), kd + 2 * k, id_s, t + k > 0 ? 1u : 0u);
-                    umma_commit(s_full(b));
-                }
-                __syncwarp();
+                    for (int k = 0; k < D / 32; ++k)
+                        umma_f8(tmem + (uint32_t)b * KP_KEYS, qd + (uint64_t)(t * L::Q_BYTES / 16 + 2 * k), kd + 2 * k, id_s, t + k > 0 ? 1u : 0u);
+                umma_commit(s_full(b));
             };
-            if (n_tiles > 0) issue_s(0);
-            if (n_tiles > 1) issue_s(1);
+            for (int j = 0; j < 2 && j < n_tiles && ok; ++j) {
+                ok = keys_of(j);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (ok && elect_lane()) issue_s(j);
+                __syncwarp();
+            }
             for (int j = 0; j < n_tiles && ok; ++j) {
                 const int s = j % KP_STAGES, b = j & 1;
-                ok = wait(p_full(b), (uint32_t)((j >> 1) & 1)) && wait(v_full(s), (uint32_t)((j / KP_STAGES) & 1));
+                // (what came long ago is waited for first: a group's weights are followed by its product at once)
+                ok = wait(v_full(s), (uint32_t)((j / KP_STAGES) & 1)) && keys_of(j + 2) && wait(p_full(b), (uint32_t)((j >> 1) & 1));
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t vd = desc8<128>(base + L::H + (uint32_t)s * L::V16);
@@ -242,13 +256,10 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
                         for (int k = 0; k < KP_KEYS / 16; ++k)       // 16 keys: 8 columns of P, 16 rows of V
                             umma_f16_ta(tmem_pv + (uint32_t)(b * D + 64 * h), tmem + (uint32_t)(b * KP_KEYS + 8 * k), vd + (uint64_t)(h * L::HALF / 16 + 128 * k),
                                         id_pv, (j > 1 || k > 0) ? 1u : 0u);
-                }
-                __syncwarp();
-                // (in order behind the product that reads P_j, where S_{j+2} goes; the group's next wait is for it, and for that product)
-                if (j + 2 < n_tiles) issue_s(j + 2);
-                // (one phase of pv_full: a group that skipped phases could not tell by a phase's one bit which is open)
-                if (elect_lane()) {
-                    if (j + 2 >= n_tiles) umma_commit(pv_full(b));
+                    // (in order behind the product that reads P_j, where S_{j+2} goes; the group's next wait is for it, and for that product)
+                    if (j + 2 < n_tiles) issue_s(j + 2);
+                    // (one phase of pv_full: a group that skipped phases could not tell by a phase's one bit which is open)
+                    else umma_commit(pv_full(b));
                     umma_commit(kv_empty(s));
                 }
                 __syncwarp();
@@ -323,24 +334,23 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
         for (int j = grp; j < n_tiles; j += 2) {
             const int turn = j >> 1, j0 = tile_j0(j), s = j % KP_STAGES;
             // (after a failed wait the loop still runs to its end, without waiting: every thread meets the barrier behind it)
-            if (ok) ok = k8_wait(s_full(grp), (uint32_t)(turn & 1)) && k8_wait(kv_full(s), (uint32_t)((j / KP_STAGES) & 1));
+            if (ok) ok = k8_wait(kv_full(s), (uint32_t)((j / KP_STAGES) & 1));
+            // (a group's scales are read when they are used, twice: the scores leave no registers to keep them in)
+            const uint32_t sc = base + L::SCALES + (uint32_t)(s * KP_GROUPS * 8);
+            auto scale_of = [&](int g) {
+                float2 f;
+                asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(f.x), "=f"(f.y) : "r"(sc + 8u * g) : "memory");
+                const float k = f.x * c_row;
+                const int bits = __float_as_int(f.y);
+                // (never 0: what is hidden is minus infinity before it is multiplied; NaN stays)
+                return make_float3(k < 1.2e-38f ? 1.2e-38f : k, __int_as_float(0x4b000000 | (bits >> 23)) - 8388735.0f, __int_as_float((254 << 23) - bits));
+            };
+            if (ok) ok = k8_wait(s_full(grp), (uint32_t)(turn & 1));
             ok = __all_sync(0xffffffffu, ok);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float x[2][32];                              // the row's 64 products stay in registers
             tmem_ld32(s_addr, x[0]);
             tmem_ld32(s_addr + 32u, x[1]);
-            const float2* sc = reinterpret_cast<const float2*>(smem_raw + L::SCALES) + s * KP_GROUPS;
-            float kc[KP_GROUPS], ev[KP_GROUPS], inv_v[KP_GROUPS];
-#pragma unroll
-            for (int g = 0; g < KP_GROUPS; ++g) {
-                const float2 f = sc[g];
-                const int bits = __float_as_int(f.y);
-                // (never 0: what is hidden is minus infinity before it is multiplied; NaN stays)
-                kc[g] = f.x * c_row;
-                kc[g] = kc[g] < 1.2e-38f ? 1.2e-38f : kc[g];
-                ev[g] = __int_as_float(0x4b000000 | (bits >> 23)) - 8388735.0f;
-                inv_v[g] = __int_as_float((254 << 23) - bits);
-            }
             // a tile every row of the CTA sees whole needs no comparisons
             if (j0 + KP_KEYS - 1 > pos_first || j0 < lo_last) {
 #pragma unroll
@@ -355,10 +365,11 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
 #pragma unroll
             for (int g = 0; g < KP_GROUPS; ++g) {
                 const float* v = &x[g >> 1][16 * (g & 1)];
-                float m4[4];
+                float m5[5];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) m4[e] = fmaxf(fmaxf(v[e], v[e + 4]), fmaxf(v[e + 8], v[e + 12]));
-                top = fmaxf(top, fmaf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), kc[g], ev[g]));
+                for (int e = 0; e < 5; ++e) m5[e] = max3(v[3 * e], v[3 * e + 1], v[3 * e + 2]);
+                const float3 f = scale_of(g);
+                top = fmaxf(top, fmaf(fmaxf(max3(m5[0], m5[1], m5[2]), max3(m5[3], m5[4], v[15])), f.x, f.y));
             }
             if (__any_sync(0xffffffffu, top > m_ref + KP_LAZY)) {
                 const float m_new = fmaxf(m_ref, top);
@@ -384,7 +395,8 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
 #pragma unroll
                 for (int gg = 0; gg < 2; ++gg) {
                     const int g = 2 * h + gg;
-                    const float2 k2 = make_float2(kc[g], kc[g]), b2 = make_float2(ev[g] + up, ev[g] + up);
+                    const float3 f = scale_of(g);
+                    const float2 k2 = make_float2(f.x, f.x), b2 = make_float2(f.y + up, f.y + up);
                     float2 sum = make_float2(0.f, 0.f), alt = sum;
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
@@ -395,7 +407,7 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
                         const __half2 p = __floats2half2_rn(w.x, w.y);
                         packed[8 * gg + (e >> 1)] = *reinterpret_cast<const uint32_t*>(&p);
                     }
-                    l_row = fmaf((sum.x + sum.y) + (alt.x + alt.y), inv_v[g], l_row);
+                    l_row = fmaf((sum.x + sum.y) + (alt.x + alt.y), f.z, l_row);
                 }
                 asm volatile(
                     "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"

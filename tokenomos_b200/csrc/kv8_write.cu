@@ -15,7 +15,8 @@
 // look for them, among `look` tokens in a row each: every token of a small step, four of a large one, most of which begin none. Queries need no run: CTAs
 // of their own take the heads of one token, or of four where there are many. Large steps take CTAs of 8 warps (two KV heads each).
 //
-// Bound by its chain of dependent loads (tokens, page, rows) at decode sizes; measured figures stand with the entry point.
+// Measured (one B200, 32 heads over 8 of 64): 8 single tokens 3.0 us, a prompt of 2,048 tokens 13.2 (3.5 us of them its bytes' at HBM's rate), three portions of 333 tokens of the
+// 32-bit model (16 heads over 8) 6.1. Bound by its chain of dependent loads (tokens, page, rows) at decode sizes, by instructions in long prompts (2.3 of 4 a cycle).
 #include <math.h>
 
 #include "kv8.cuh"
