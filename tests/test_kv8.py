@@ -224,6 +224,38 @@ def test_write_follows_the_definition_however_the_tokens_are_cut(dtype, H, G, D,
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("H, G, D, P", [(2, 1, 64, 16), (16, 8, 64, 16), (9, 3, 128, 7), (8, 8, 64, 64)])
+def test_a_large_step_writes_what_small_ones_write(dtype, H, G, D, P):
+    """Steps of 512 tokens and more look for their runs and share their heads out otherwise: the same bits all the same, in pages that are new and
+    in pages that hold earlier tokens, whatever the runs' lengths and places."""
+    g = torch.Generator().manual_seed(D + P)
+    firsts = torch.randint(0, 40, (70,), generator=g).tolist()
+    counts = (torch.randint(1, 4, (70,), generator=g) ** 4).tolist()          # 1, 16 and 81
+    counts[5], counts[41] = 700, 333
+    lens = [a + n for a, n in zip(firsts, counts)]
+    freq = torch.exp(-torch.arange(D // 2) * 0.2).cuda()
+    wq, wk = (torch.rand(2, D, generator=g) + 0.5).cuda()
+    before = [torch.randn(a, (H + 2 * G) * D, generator=g).cuda().to(dtype) for a in firsts]
+    rows = [(torch.randn(n, (H + 2 * G) * D, generator=g) * 4).cuda().to(dtype) for n in counts]
+    assert sum(counts) >= 512 and sum(firsts) >= 512
+    large, small = Cache(lens, G, D, P), Cache(lens, G, D, P)
+    for part, at in ((before, [0] * 70), (rows, firsts)):
+        step = [(s, a, x) for s, (a, x) in enumerate(zip(at, part)) if len(x)]
+        q, _ = write(large, step, H, wq, wk, 1e-6, freq)
+        got = []
+        for s, a, x in step:                                                   # (whole pages' runs, fewer than 512 tokens)
+            i = 0
+            while i < len(x):
+                n = min(len(x) - i, (P - (a + i) % P) + 400 // P * P)
+                got.append(write(small, [(s, a + i, x[i:i + n])], H, wq, wk, 1e-6, freq)[0])
+                i += n
+        assert torch.equal(q, torch.cat(got))
+        assert torch.equal(large.pool.view(torch.uint8), small.pool.view(torch.uint8))
+        assert torch.equal(large.scales.view(torch.int32), small.scales.view(torch.int32))
+
+
+@gpu
 def test_a_block_that_grows_rescales_what_it_holds():
     """Tokens of rising size, one a step: the earlier bytes follow the scale exactly while they are normal numbers."""
     G, D, P = 2, 64, 16

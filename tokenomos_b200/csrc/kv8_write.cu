@@ -12,12 +12,14 @@
 // A block (page, K|V, head) has one writer: the tokens of a sequence that fall into one page within a step form a run, and four warps of one CTA take a
 // run's keys and values of one KV head (a block's maximum then needs no atomics, and the bytes do not depend on which warp came first). They hold 16
 // tokens in registers (8 for heads of 128) between the maximum and the bytes; a longer run is read again, from L1. Runs begin where the CTAs
-// look for them, among `look` tokens in a row each: every token of a small step, four of a large one, most of which begin none. Queries need no run: CTAs
+// look for them, among `look` tokens in a row each: one of a small step, 4 to 16 of a large one. Queries need no run: CTAs
 // of their own take the heads of one token, or of four where there are many. Large steps take CTAs of 8 warps (two KV heads each).
 //
-// Measured (one B200, 32 heads over 8 of 64): 8 single tokens 3.0 us, a prompt of 2,048 tokens 13.2 (3.5 us of them its bytes' at HBM's rate), three portions of 333 tokens of the
-// 32-bit model (16 heads over 8) 6.1. Bound by its chain of dependent loads (tokens, page, rows) at decode sizes, by instructions in long prompts (2.3 of 4 a cycle).
+// Measured (one B200, 32 heads over 8 of 64): 8 single tokens 3.0 us, a prompt of 2,048 tokens 11.4 (3.5 us of them its bytes' at HBM's rate), three portions of 333 tokens of the
+// 32-bit model (16 heads over 8) 5.4. Bound by its chain of dependent loads (tokens, page, rows) at decode sizes, by instructions in long prompts (2.3 of 4 a cycle).
 #include <math.h>
+
+#include <algorithm>
 
 #include "kv8.cuh"
 
@@ -335,7 +337,11 @@ TK_API int tk_qk_norm_rope_write8(const void* qkv, int64_t qkv_stride, void* q_o
     // (a prompt of 2,048 tokens, 32 heads over 8 of 64, us by warps a CTA: 15.7 with 4, 13.2 with 8, 13.9 with 16; three portions of 333 of the 32-bit
     // model 6.9, 6.1, 6.8; eight single tokens 3.0 with 4)
     const bool many = T_ >= 512;
-    const int warps = many ? 8 : 4, look = many ? 4 : 1, q_tokens = many ? 4 : 1;
+    // Of a large step's keys and values a CTA takes as many tokens as leave about four CTAs an SM, but 4 at least (a step of single tokens has a run each) and 16 at
+    // most (a page; us with 4 tokens, 16, and so: the prompt of 2,048 13.3, 10.8, 11.4; 8,192 49.9, 41.0, 41.0; three portions of 333 6.2, 6.8, 5.4; 600 single tokens 18.7,
+    // 38.7, 16.8).
+    const int warps = many ? 8 : 4, q_tokens = many ? 4 : 1;
+    const int look = many ? (int)std::clamp<int64_t>((int64_t)T_ * ceil_div(Hkv, warps / 4) / (4 * 148) + 1, 4, 16) : 1;
     const int q_ctas = many ? 1 : ceil_div(H, warps * 32 / (D / 8));
     const int64_t kv_blocks = (int64_t)ceil_div(T_, look) * ceil_div(Hkv, warps / 4), blocks = kv_blocks + (int64_t)ceil_div(T_, q_tokens) * q_ctas;
     TK_CHECK_ARG(blocks < 0x7fffffff, "qk_norm_rope_write8: %d tokens are too many", T_);
