@@ -196,6 +196,15 @@ def test_models_and_layers_without_an_8_bit_form_are_refused(tmp_path):
         models.configure(folder, cache="int4")
 
 
+def test_a_cache_type_beside_a_configured_model_is_refused(tmp_path):
+    from tokenomos_b200 import LLM, models
+    from tokenomos_b200.weights import write_model_folder
+
+    write_model_folder(tmp_path / "d", TINY_D, 0, 0.02, 0.0, torch.bfloat16)
+    with pytest.raises(ValueError, match="configured already"):
+        LLM(tmp_path / "d", "cpu", models.configure(tmp_path / "d"), cache="fp8")
+
+
 @pytest.mark.parametrize("option, value", [("keep_first", 2), ("v_is_k", True), ("v_dim", 32), ("pointwise", {}), ("value_mix", {"source": None})])
 def test_attention_options_without_an_8_bit_form_are_refused(option, value):
     from tokenomos_b200.parts.attention import build_attention

@@ -91,6 +91,8 @@ class LLM:
         alone picks the work dtype (``bf16``, the default, or ``fp32``), ``cache="fp8"`` an 8-bit cache of keys and
         values. Every other keyword goes to ``Engine``: ``slots``, ``page``, ``max_len``, ``pages``, ``prefill_budget``,
         ``graphs``, ``warmup``."""
+        if arch is not None and cache is not None:
+            raise ValueError("arch is configured already: give cache to models.configure")
         self.path = Path(model)
         self._device = torch.device(device)
         self.model = models.load(model, device, arch or models.configure(model, work=work, cache=cache))
