@@ -14,7 +14,8 @@
 // interleave (prmt) into the pairs that a fragment holds. e4m3 is exact in float16.
 //
 // What is rounded: q (bfloat16: not at all, 32-bit: to 22 bits, as two float16 with two products) after division by a power of two that brings its row
-// to [2^14, 2^15), so that its small elements keep their bits; the weights to float16's 11 bits (32-bit: 22, as two). Scores, the running
+// to [2^14, 2^15), so that its small elements keep their bits; the weights (of the bytes) to float16's 11 bits (32-bit: 22,
+// as two) or, where that is more, to 2^-32 of the row's largest: half of float16's smallest step against 2^7, which that one has at least. Scores, the running
 // maximum, sums and outputs are 32-bit; the output is rounded once.
 //
 // A value block's scale joins the exponent: with x_j = log2(p_j) + log2(s_V), w_j = 2^(x_j - m + 7) are the weights of the bytes, m following their
