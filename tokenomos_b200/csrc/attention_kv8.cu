@@ -19,8 +19,8 @@
 // maximum, sums and outputs are 32-bit; the output is rounded once.
 //
 // A value block's scale joins the exponent: with x_j = log2(p_j) + log2(s_V), w_j = 2^(x_j - m + 7) are the weights of the bytes, m following their
-// running maximum lazily (it is raised when a row exceeds it by 8, so w <= 2^15), and the softmax's sum is of w_j / s_V. No weight then
-// loses bits to float16's range against a larger one, however far apart the blocks' scales are.
+// running maximum lazily (it is raised when a row exceeds it by 8, so w <= 2^15), and the softmax's sum is of w_j / s_V. A weight
+// then loses bits to float16's range only beside one that gives the output that much more a byte, however far apart the blocks' scales are.
 //
 // Masked keys and values are never read (their bytes are zero in the products), so what an unwritten part of a page holds does not
 // matter. A row that sees no key is 0.
