@@ -24,7 +24,9 @@
 // Measured (one B200, pages of 16): one token behind 2,048 positions 7.7 us and 64 behind up to 3,000 33.1 (32 heads over 8 of 64; 9.9 and 69 on mma.sync), 8
 // behind 32,000 45.5 (16 heads over 8: 5.7 TB/s; 109), 16 behind a window of 1,024 9.5 (16 heads over 4 of 128; 16.3). Long contexts come near HBM; below
 // some 8 MB of cache the launch, the chain of a tile's products and weights and the shares' joining are what there is. Tried and slower or no faster: two or four to six tiles
-// ahead, four copying warps or one (65-100 cycles a load, one after the other within a warp), the shares joined through global memory.
+// ahead, four copying warps or one (65-100 cycles a load, one after the other within a warp), the shares joined through global memory,
+// CTAs that stay and take one unshared token and KV head after the other, their loads and q running ahead (512 behind up to 300: 59 became 49, but 128 behind up
+// to 4,000 75 became 81 and 128 behind up to 500 18.3 became 20.5).
 //
 // Masking and sums are those of attention_kv8.cu; every wait is bounded (about a second), the kernel then frees its tensor memory and
 // returns, and tk_attn_kv8_status() says so.
