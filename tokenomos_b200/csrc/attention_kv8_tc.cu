@@ -95,7 +95,7 @@ struct K8tSmem {
     static constexpr int STAGES = k8t_stages<D>;
     static constexpr int S_COLS = 2 * NR < 16 ? 16 : 2 * NR;                       // scores' columns: term, head
     static constexpr int O_COLS = 4 * NR < 16 ? 16 : 4 * NR;                       // outputs' columns: term, head
-    static constexpr int P_BYTES = O_COLS * K8T_KEYS;                              // [term, head][key], 128-byte swizzle
+    static constexpr int P_BYTES = O_COLS * K8T_KEYS;                              // [term, head / 16][key][16]
     static constexpr int P = 0;                                                    // two of them
     static constexpr int Q = 2 * P_BYTES;                                          // [term, head][d]
     static constexpr int KV = Q + (S_COLS * D < 1024 ? 1024 : S_COLS * D);         // stages: K tile, V tile
@@ -109,6 +109,12 @@ struct K8tSmem {
     static_assert(NR * (D + 2) * 4 <= STAGES * STAGE, "a share");
     static_assert(Q % 1024 == 0 && KV % 1024 == 0, "swizzled tiles");
 };
+
+// The weights' terms as the second product's other operand: 16 of them (bytes) a key, keys one after the other, further ones K8T_KEYS keys on. MN-major
+// without swizzle: eight keys are 128 bytes, the next eight follow.
+__device__ __forceinline__ uint64_t desc_keys16(uint32_t at) {
+    return (uint64_t)((at & 0x3FFFF) >> 4) | (uint64_t)(128 >> 4) << 16 | (uint64_t)(16 * K8T_KEYS >> 4) << 32 | (uint64_t)1 << 46;
+}
 
 // D: head size; NR: query heads a KV head has, rounded up to 2, 4, 8 or 16
 template <int D, int NR>
@@ -262,7 +268,7 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
         }
     } else if (warp == K8T_MMA_WARP) {
         // ---- the products ----
-        constexpr uint32_t id_s = idesc8(K8T_KEYS, L::S_COLS, false), id_o = idesc8(D, L::O_COLS, true);
+        constexpr uint32_t id_s = idesc8(K8T_KEYS, L::S_COLS, false), id_o = idesc8(D, L::O_COLS, true) | 1u << 16;
         const uint64_t qd = desc8<D>(base + L::Q);
         auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, k8_wait(bar, parity)) != 0; };
         bool ok = true;
@@ -289,11 +295,11 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint64_t vd = desc8<D>(base + L::KV + (uint32_t)s * L::STAGE + K8T_KEYS * D);
-            const uint64_t pd = desc8<128>(base + L::P + b * L::P_BYTES);
+            const uint64_t pd = desc_keys16(base + L::P + b * L::P_BYTES);
             if (elect_lane()) {
 #pragma unroll
                 for (int k = 0; k < K8T_KEYS / 32; ++k)
-                    umma_f8(tmem_o, vd + (uint64_t)(k * 32 * D / 16), pd + 2 * k, id_o, j + k > 0 ? 1u : 0u);
+                    umma_f8(tmem_o, vd + (uint64_t)(k * 32 * D / 16), pd + 32 * k, id_o, j + k > 0 ? 1u : 0u);
                 umma_commit(pv_full(b));
                 umma_commit(kv_empty(s));
             }
@@ -301,12 +307,12 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
         }
     } else {
         // ---- the weights ----
-        float c[NR], m[NR], l[NR];
+        float c[NR], m[NR], l[NR], up[NR], limit[NR];         // (of a row without a maximum yet: nothing above is small enough)
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             c[r] = row_factor[r];
-            m[r] = -INFINITY;
-            l[r] = 0.f;
+            m[r] = limit[r] = -INFINITY;
+            l[r] = up[r] = 0.f;
         }
         const uint32_t lanes = (uint32_t)(warp * 32) << 16;
         bool ok = true;
@@ -320,7 +326,7 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
             const int bits = __float_as_int(sc.y);
             const float ev = __int_as_float(0x4b000000 | (bits >> 23)) - 8388735.0f, inv_v = __int_as_float((254 << 23) - bits);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            float x[NR];
+            float x[NR], y[NR];
             {
                 constexpr int N = 2 * NR < 8 ? 8 : 2 * NR;
                 float sum[N];
@@ -328,16 +334,18 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
 #pragma unroll
                 for (int r = 0; r < NR; ++r) x[r] = sum[r] + sum[NR + r];
             }
+            // the weights' logarithms
+            auto weigh = [&](int r) { y[r] = seen ? fmaf(x[r], sc.x * c[r], ev + up[r]) : -INFINITY; };
             bool above = false;
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-                x[r] = seen ? fmaf(x[r], sc.x * c[r], ev) : -INFINITY;
-                above = above || x[r] > m[r] + K8T_LAZY;
+                weigh(r);
+                above = above || y[r] > limit[r];
             }
             if (any_of_128(above)) {
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
-                    const float top = warp_max(x[r]);
+                    const float top = warp_max(y[r] - up[r]);
                     if (lane == 0) by_warp[warp * 16 + r] = top;
                 }
                 sync_128();
@@ -349,6 +357,9 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
                     f[r] = m_new == -INFINITY ? 1.f : k8_exp2(m[r] - m_new);
                     m[r] = m_new;
                     l[r] *= f[r];
+                    up[r] = m_new == -INFINITY ? 0.f : K8T_LIFT - m_new;
+                    limit[r] = m_new == -INFINITY ? -INFINITY : K8T_LIFT + K8T_LAZY;
+                    weigh(r);
                 }
                 if (it > 0) {
                     // what this warp's lanes have accumulated (no product is under way once the last tile's is done)
@@ -365,13 +376,16 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
             }
             // the terms of tile it - 2 have been read
             if (ok && it >= 2) ok = k8_wait(pv_full(b), (uint32_t)((turn - 1) & 1));
-            unsigned char* p = smem_raw + L::P + b * L::P_BYTES + (tid & 15);
+            constexpr int WORDS = L::O_COLS / 4;
+            uint32_t terms[WORDS];
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) terms[i] = 0;
 #pragma unroll
             for (int r = 0; r < NR; r += 2) {
                 float w[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    w[h] = k8_exp2(x[r + h] + (m[r + h] == -INFINITY ? 0.f : K8T_LIFT - m[r + h]));
+                    w[h] = k8_exp2(y[r + h]);
                     l[r + h] = fmaf(w[h], inv_v, l[r + h]);
                 }
                 __half2 left = __floats2half2_rn(w[0], w[1]);        // (what a term leaves of a float16 is one)
@@ -379,13 +393,15 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
                 for (int t = 0; t < K8T_PTERMS; ++t) {
                     uint16_t two;
                     asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(two) : "r"(*reinterpret_cast<const uint32_t*>(&left)));
-                    p[swizzled<128>(t * NR + r, tid >> 4)] = (unsigned char)two;
-                    p[swizzled<128>(t * NR + r + 1, tid >> 4)] = (unsigned char)(two >> 8);
+                    terms[(t * NR + r) / 4] |= (uint32_t)two << (8 * ((t * NR + r) & 2));
                     const uint32_t back = e4m3x2_to_half2(two);
                     left = __hsub2(left, *reinterpret_cast<const __half2*>(&back));
                     if (t == 1) left = __hmul2(left, __float2half2_rn(K8T_FINE));
                 }
             }
+            unsigned char* p = smem_raw + L::P + b * L::P_BYTES + tid * 16;
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 4) *reinterpret_cast<uint4*>(p + i * 4 * K8T_KEYS) = make_uint4(terms[i], terms[i + 1], terms[i + 2], terms[i + 3]);
             if (!seen) {
                 // whatever the cache (or an earlier tile) has left there
                 uint4* row = reinterpret_cast<uint4*>(smem_raw + L::KV + (it % STAGES) * L::STAGE + K8T_KEYS * D + tid * D);
