@@ -71,11 +71,12 @@ def attend(q, kv, pos, window, scale, sv, sink=False):
     return o, size, (reach, left, rest)
 
 
-def within(got, want, size, reach, keys, dtype):
+def within(got, want, size, reach, keys, dtype, least=0.0):
     """The kernel's bound. A weight's relative error: its score (D products in 32-bit sums, a few roundings of a number of at most
     `reach` log2(e): (D + 8) 2^-24 of it, and for 32-bit q 2^-22 from its two halves), the exponential's 2^-22, its rounding to
     float16 (2^-11; as two float16 2^-22; as four e4m3 terms 2^-16) and, in terms, what they leave (``attend``); the same for the sum; sums over
-    keys in 32 bits, each term's products their own; one rounding of the result."""
+    keys in 32 bits, each term's products their own; one rounding of the result. `least`: of the row's largest weight, what a 32-bit row's weights
+    are rounded to where that is more."""
     D = want.shape[-1]
     unit = torch.finfo(dtype).eps / 2
     reach, left, rest = reach
@@ -86,6 +87,8 @@ def within(got, want, size, reach, keys, dtype):
     bound = unit * want.abs() * 1.01 + size * (2 * eps + half + 8 * (keys + 64) * 2.0 ** -24) + 2.0 ** -120
     if dtype == torch.bfloat16:
         bound = bound + rest
+    else:
+        bound = bound + rest * 2.0 ** 24 * least
     off = (got.double() - want).abs()
     assert torch.isfinite(got).all()
     assert (off <= bound).all(), ((off / bound).max().item(), off.max().item())
@@ -444,6 +447,29 @@ def test_many_small_weights_beside_a_large_one(dtype):
     within(out, want, sz, reach, n, dtype)
     # (a tenth of the weights lost would move the mean of 8,000 random values by about as much)
     assert ((out.double() - want).norm() / want.norm()).item() < 0.01
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 30])
+@pytest.mark.parametrize("P", [16, 12])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("below", [8, 20, 30, 45])
+def test_weights_far_below_one_that_meets_zero_bytes(dtype, P, new, below):
+    """The first key's weight is 2^below times any other's and its value is 0. Two float16 terms of a weight end at half of float16's smallest step,
+    2^-25, while the row's largest weight is 2^7 at least: what is lost of a 32-bit row's weight is 2^-22 of it (`within`) or 2^-32 of the largest."""
+    n = 300
+    cache = Cache([n], 1, 64, P).fill(seed=below)
+    raw = cache.pool.view(torch.uint8)
+    raw[cache.table[0].long().cuda(), 0, 0] = 0
+    raw[int(cache.table[0, 0]), :, 0, 0] = 0
+    cache.pool[int(cache.table[0, 0]), 0, 0, 0, 0] = torch.tensor(256.0).to(F8)
+    cache.scales[:] = 2.0 ** -7
+    q = torch.zeros(new, 4, 64, device="cuda", dtype=dtype)
+    q[:, :, 0] = 4.0
+    scale = below * math.log(2.0) / (4.0 * 2.0)
+    out, pos = run_attention(cache, q, [new], None, scale)
+    want, sz, reach = attend(q.double(), cache.of(0), pos, None, scale, cache.value_scales(0))
+    within(out, want, sz, reach, n, dtype, least=2.0 ** -32)
 
 
 @gpu
