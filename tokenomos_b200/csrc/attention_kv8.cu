@@ -446,10 +446,9 @@ TK_API int tk_attn_kv8_supported(int H, int Hkv, int D) {
     return Hkv > 0 && H > 0 && H % Hkv == 0 && H / Hkv <= K8_ROWS && (D == 64 || D == 128);
 }
 
-// Whether prompt portions of this shape take the tcgen05 kernel: 16-bit, a group that divides 128, pages that are a power of two and 16 or more
-// positions.
+// Whether prompt portions of this shape take the tcgen05 kernel: 16-bit, pages that are a power of two and 8 or more positions.
 TK_API int tk_attn_kv8_prefill_supported(int H, int Hkv, int D, int P, int dtype) {
-    return tk_attn_kv8_supported(H, Hkv, D) && dtype == TK_BF16 && 128 % (H / Hkv) == 0 && P >= 16 && (P & (P - 1)) == 0;
+    return tk_attn_kv8_supported(H, Hkv, D) && dtype == TK_BF16 && P >= 8 && (P & (P - 1)) == 0;
 }
 
 // Tokens of one sequence a tile of tk_attn_kv8 has.
@@ -499,8 +498,8 @@ TK_API int tk_attn_kv8_splits(int items, int H, int Hkv, int D, int longest, int
     return (int)(n < 1 ? 1 : n);
 }
 
-// Whether single tokens of this shape take the tcgen05 kernel: 16-bit queries, pages that are a power of two and 16 or more positions.
-TK_API int tk_attn_kv8_single_tc(int P, int dtype) { return dtype == TK_BF16 && P >= 16 && (P & (P - 1)) == 0; }
+// Whether single tokens of this shape take the tcgen05 kernel: 16-bit queries, pages that are a power of two and 8 or more positions.
+TK_API int tk_attn_kv8_single_tc(int P, int dtype) { return dtype == TK_BF16 && P >= 8 && (P & (P - 1)) == 0; }
 
 int tk_attn_kv8_tc(const void* q, const void* pool, const float* scales, void* out, const void* args, int D, cudaStream_t stream);
 int tk_attn_kv8_tc_status();

@@ -4,7 +4,7 @@
 //                  multiplied one after the other into the same accumulator
 //   O += P V       kind::f16, P float16 in tensor memory where S was, V's bytes turned into float16 on the way (e4m3 is exact in it)
 //
-// A CTA takes up to 128 rows: 128 / G tokens of one sequence with the G query heads that share one KV head (row = token * G + head), and walks the keys
+// A CTA takes up to 128 rows: 128 / G tokens (rounded down) of one sequence with the G query heads that share one KV head (row = token * G + head), and walks the keys
 // in tiles of 64, this step's own included. Warps coupled by mbarriers only:
 //
 //   warp 0      brings K and V by TMA, a page (or 64 positions of one) a load, up to five tiles ahead, and the tiles' scales
@@ -13,7 +13,7 @@
 //   warps 4-11  bring q's terms, then are two groups of 128 threads that take the key tiles in turn, each with scores, weights and an output of
 //               its own, so that one's chain runs under the other's; thread r owns row r of its group's tiles
 //
-// A tile's 64 keys lie in four groups of 16 with one scale for keys and one for values each (pages are 16 positions or more). With c = scale log2(e)
+// A tile's 64 keys lie in four groups of 16 (or eight of 8, for pages of 8) with one scale for keys and one for values each. With c = scale log2(e)
 // and x_j = s_K c (q . kb_j) + log2(s_V), the weight of a value's bytes is 2^(x_j - m + 7) and the softmax's sum adds those weights over s_V, a group at a
 // time: a score costs one multiply-add and one exponential, as without scales. m follows the running maximum lazily (raised when a row exceeds it
 // by 8: weights stay below 2^15 of float16's 65,504, and reach down to 2^-31 of the row's largest); only then is the output read, scaled and
@@ -39,22 +39,23 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int KP_ROWS = 128, KP_KEYS = 64, KP_GROUPS = KP_KEYS / 16;
+constexpr int KP_ROWS = 128, KP_KEYS = 64;
 constexpr int KP_THREADS = 384;
 constexpr int KP_STAGES = 5;
 constexpr int KP_SPLIT_TILES = 8;                          // key tiles a CTA should have before a tile's keys are shared out
 constexpr float KP_LAZY = 8.0f, KP_LIFT = 7.0f;
 
-// shared memory of a CTA: two fit an SM for heads of 64, one for heads of 128
-template <int D>
+// shared memory of a CTA: two fit an SM for heads of 64, one for heads of 128. KG: keys that share scales, 16, or 8 where a page has no more.
+template <int D, int KG>
 struct KpSmem {
+    static constexpr int GROUPS = KP_KEYS / KG;
     static constexpr int Q_BYTES = KP_ROWS * D;            // of a term
     static constexpr int RAW = KP_KEYS * D;                // keys' or values' bytes of a tile
     static constexpr int HALF = KP_KEYS * 128;             // float16 values of a tile, 64 columns
     static constexpr int V16 = HALF * (D / 64);
     static constexpr int Q = 0, K = 2 * Q_BYTES, V = K + KP_STAGES * RAW, H = V + KP_STAGES * RAW;
     static constexpr int SCALES = H + KP_STAGES * V16;     // [stage][group] (key's, value's)
-    static constexpr int FACTOR = SCALES + KP_STAGES * KP_GROUPS * 8;
+    static constexpr int FACTOR = SCALES + KP_STAGES * GROUPS * 8;
     static constexpr int BARS = FACTOR + KP_ROWS * 4;
     static constexpr int BYTES = BARS + (3 * KP_STAGES + 7) * 8 + 16;
     static constexpr int SHARE_LD = D + 4;
@@ -79,10 +80,11 @@ __device__ __forceinline__ void umma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, ui
         : "memory");
 }
 
-template <int D>
+template <int D, int KG>
 __global__ void __launch_bounds__(KP_THREADS, D == 64 ? 2 : 1)
 attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* out, const __grid_constant__ CUtensorMap map, const K8Args a) {
-    using L = KpSmem<D>;
+    using L = KpSmem<D, KG>;
+    constexpr int GROUPS = L::GROUPS, AHEAD = 32 / GROUPS;         // tiles whose pages and scales the copying warp's lanes know
     constexpr uint32_t COLS = D == 64 ? 256 : 512;         // tensor memory: two of 64 columns for scores, two of D for outputs
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     pdl_launch_dependents();
@@ -151,12 +153,12 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
     if (warp < 4) {
         if constexpr (D == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         if (warp == 0) {
-            // lane i knows the page and the scales of 16 positions of one of eight tiles, and brings the page (or 64 positions of it) if they are its
-            // first of the tile; asked for 16 and 8 tiles ahead
-            const int per = 1 << min(a.p_shift, 6), group = lane & 3, at_row = (group * 16) & (per - 1);
+            // lane i knows the page and the scales of KG positions of one of eight tiles (KG = 8: four), and brings the page (or 64 positions of it) if
+            // they are its first of the tile; asked for 16 and 8 (8 and 4) tiles ahead
+            const int per = 1 << min(a.p_shift, 6), group = lane & (GROUPS - 1), at_row = (group * KG) & (per - 1);
             bool ok = true;
-            auto page_of = [&](int eight) {
-                const int it = eight * 8 + (lane >> 2), j = tile_j0(it) + group * 16 - at_row;
+            auto page_of = [&](int block) {
+                const int it = block * AHEAD + lane / GROUPS, j = tile_j0(it) + group * KG - at_row;
                 return it < n_tiles && j <= pos_last && j + per > lo ? TK_PAGE(TK_K_KV8_ATTN, bt_row[j >> a.p_shift]) : -1;
             };
             auto scales_of = [&](int pg) {
@@ -168,24 +170,24 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
             float2* sc = reinterpret_cast<float2*>(smem_raw + L::SCALES);
             for (int it = 0; it < n_tiles; ++it) {
                 const int s = it % KP_STAGES;
-                if ((it & 7) == 0) {
+                if (it % AHEAD == 0) {
                     page = page_next;
                     scale = scale_next;
                     page_next = page_after;
                     scale_next = scales_of(page_next);
-                    page_after = page_of(it / 8 + 2);
+                    page_after = page_of(it / AHEAD + 2);
                 }
                 if (it >= KP_STAGES) ok = k8_wait(kv_empty(s), (uint32_t)((it / KP_STAGES - 1) & 1));
                 if (!__all_sync(0xffffffffu, ok)) break;
-                const bool ours = (lane >> 2) == (it & 7), mine = ours && page >= 0 && at_row == 0;
+                const bool ours = lane / GROUPS == it % AHEAD, mine = ours && page >= 0 && at_row == 0;
                 const int loads = __popc(__ballot_sync(0xffffffffu, mine));
                 if (mine) {
-                    const int row = (page * 2 * Hkv + kvh) * P + ((tile_j0(it) + group * 16) & (P - 1));
-                    const uint32_t at = base + (uint32_t)(s * L::RAW + group * 16 * D);
+                    const int row = (page * 2 * Hkv + kvh) * P + ((tile_j0(it) + group * KG) & (P - 1));
+                    const uint32_t at = base + (uint32_t)(s * L::RAW + group * KG * D);
                     tma_load_2d(at + L::K, &map, 0, row, kv_full(s));
                     tma_load_2d(at + L::V, &map, 0, row + Hkv * P, kv_full(s));
                 }
-                if (ours) sc[s * KP_GROUPS + group] = scale;
+                if (ours) sc[s * GROUPS + group] = scale;
                 __syncwarp();
                 // (the phase ends with this arrival and the bytes, whichever come last)
                 if (lane == 0) mbar_expect_tx(kv_full(s), (uint32_t)(loads * 2 * per * D));
@@ -268,14 +270,13 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
         __syncwarp();
     } else {
         if constexpr (D == 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
-        const int g_shift = __ffs(G) - 1;
         {
             // ---- q's terms: a row two threads (rows past the tile are zero) ----
             const int rr = (tid - 128) >> 1, c0 = (tid & 1) * (D / 2);
             uint4 raw[D / 16];
             float big = 0.f;
             bool fine = true;
-            const __nv_bfloat16* src = q + ((size_t)(tok0 + (rr >> g_shift)) * H + kvh * G + (rr & (G - 1))) * D + c0;
+            const __nv_bfloat16* src = q + ((size_t)(tok0 + rr / G) * H + kvh * G + rr % G) * D + c0;
 #pragma unroll
             for (int e = 0; e < D / 16; ++e) {
                 raw[e] = make_uint4(0u, 0u, 0u, 0u);
@@ -325,7 +326,7 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
         const int grp = (warp - 4) >> 2, r = (tid - 128) & 127, quarter = warp & 3;
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
         const uint32_t out_addr = tmem_pv + (uint32_t)grp * D + lane_base;
-        const int pos_r = r < rows ? pos_first + (r >> g_shift) : -1;
+        const int pos_r = r < rows ? pos_first + r / G : -1;
         const int lo_r = first_seen(pos_r, a.window), lo_last = first_seen(pos_last, a.window);
         const float c_row = row_factor[r];
         const uint32_t s_addr = tmem + lane_base + (uint32_t)grp * KP_KEYS;
@@ -336,7 +337,7 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
             // (after a failed wait the loop still runs to its end, without waiting: every thread meets the barrier behind it)
             if (ok) ok = k8_wait(kv_full(s), (uint32_t)((j / KP_STAGES) & 1));
             // (a group's scales are read when they are used, twice: the scores leave no registers to keep them in)
-            const uint32_t sc = base + L::SCALES + (uint32_t)(s * KP_GROUPS * 8);
+            const uint32_t sc = base + L::SCALES + (uint32_t)(s * GROUPS * 8);
             auto scale_of = [&](int g) {
                 float2 f;
                 asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(f.x), "=f"(f.y) : "r"(sc + 8u * g) : "memory");
@@ -363,13 +364,13 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
             }
             float top = -INFINITY;
 #pragma unroll
-            for (int g = 0; g < KP_GROUPS; ++g) {
-                const float* v = &x[g >> 1][16 * (g & 1)];
-                float m5[5];
-#pragma unroll
-                for (int e = 0; e < 5; ++e) m5[e] = max3(v[3 * e], v[3 * e + 1], v[3 * e + 2]);
+            for (int g = 0; g < GROUPS; ++g) {
+                const float* v = &x[g * KG / 32][g * KG % 32];
+                float most = fmaxf(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]));
+                most = max3(most, v[6], v[7]);
+                if constexpr (KG == 16) most = max3(most, max3(max3(v[8], v[9], v[10]), v[14], v[15]), max3(v[11], v[12], v[13]));
                 const float3 f = scale_of(g);
-                top = fmaxf(top, fmaf(fmaxf(max3(m5[0], m5[1], m5[2]), max3(m5[3], m5[4], v[15])), f.x, f.y));
+                top = fmaxf(top, fmaf(most, f.x, f.y));
             }
             if (__any_sync(0xffffffffu, top > m_ref + KP_LAZY)) {
                 const float m_new = fmaxf(m_ref, top);
@@ -393,19 +394,19 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
             for (int h = 0; h < 2; ++h) {
                 uint32_t packed[16];
 #pragma unroll
-                for (int gg = 0; gg < 2; ++gg) {
-                    const int g = 2 * h + gg;
+                for (int gg = 0; gg < 32 / KG; ++gg) {
+                    const int g = 32 / KG * h + gg;
                     const float3 f = scale_of(g);
                     const float2 k2 = make_float2(f.x, f.x), b2 = make_float2(f.y + up, f.y + up);
                     float2 sum = make_float2(0.f, 0.f), alt = sum;
 #pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        const float2 y = __ffma2_rn(make_float2(x[h][16 * gg + e], x[h][16 * gg + e + 1]), k2, b2);
+                    for (int e = 0; e < KG; e += 2) {
+                        const float2 y = __ffma2_rn(make_float2(x[h][KG * gg + e], x[h][KG * gg + e + 1]), k2, b2);
                         const float2 w = make_float2(k8_exp2(y.x), k8_exp2(y.y));
                         if (e & 2) alt = __fadd2_rn(alt, w);
                         else sum = __fadd2_rn(sum, w);
                         const __half2 p = __floats2half2_rn(w.x, w.y);
-                        packed[8 * gg + (e >> 1)] = *reinterpret_cast<const uint32_t*>(&p);
+                        packed[KG / 2 * gg + (e >> 1)] = *reinterpret_cast<const uint32_t*>(&p);
                     }
                     l_row = fmaf((sum.x + sum.y) + (alt.x + alt.y), f.z, l_row);
                 }
@@ -438,7 +439,7 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
             const float f0 = k8_factor(m_ref, l_row, m_all), f1 = k8_factor(theirs.x, theirs.y, m_all);
             l_row = two ? fmaf(l_row, f0, theirs.y * f1) : l_row;
             m_ref = m_all;
-            const int tok = tok0 + (r >> g_shift), head = kvh * G + (r & (G - 1));
+            const int tok = tok0 + r / G, head = kvh * G + r % G;
             __nv_bfloat16* dst = out + ((size_t)tok * H + head) * D;
             float inv = 1.f, gate = 1.f;
             if (nsplit == 1) {
@@ -531,31 +532,31 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
     }
 }
 
-template <int D>
+template <int D, int KG>
 cudaError_t kp_launch(const void* q, const float* scales, void* out, const CUtensorMap& map, const K8Args& a, cudaStream_t stream) {
     static std::atomic<uint64_t> done{0};
-    const cudaError_t e = k8_allow(attn_kv8_prefill_kernel<D>, KpSmem<D>::BYTES, false, done);
+    const cudaError_t e = k8_allow(attn_kv8_prefill_kernel<D, KG>, KpSmem<D, KG>::BYTES, false, done);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.items * a.Hkv * a.nsplit));
     cfg.blockDim = dim3(KP_THREADS);
-    cfg.dynamicSmemBytes = KpSmem<D>::BYTES;
+    cfg.dynamicSmemBytes = KpSmem<D, KG>::BYTES;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
     cfg.numAttrs = k8_attributes(attr, a.nsplit);
-    return cudaLaunchKernelEx(&cfg, attn_kv8_prefill_kernel<D>, (const __nv_bfloat16*)q, scales, (__nv_bfloat16*)out, map, a);
+    return cudaLaunchKernelEx(&cfg, attn_kv8_prefill_kernel<D, KG>, (const __nv_bfloat16*)q, scales, (__nv_bfloat16*)out, map, a);
 }
 
 }  // namespace
 
-// The arguments of tk_attn_kv8 for tiles (attention_kv8.cu checks them): bfloat16, a group of query heads that divides 128, pages that are a power of two
-// and 16 or more.
+// The arguments of tk_attn_kv8 for tiles (attention_kv8.cu checks them): bfloat16, pages that are a power of two and 8 or more.
 int tk_attn_kv8_prefill_tc(const void* q, const void* pool, const float* scales, void* out, const void* args, int D, cudaStream_t stream) {
     const K8Args& a = *static_cast<const K8Args*>(args);
     CUtensorMap map = {};
     TK_CHECK_ARG(k8_map(&map, pool, D, a.P < KP_KEYS ? a.P : KP_KEYS), "attn_kv8: cuTensorMapEncodeTiled failed");
-    const cudaError_t e = D == 64 ? kp_launch<64>(q, scales, out, map, a, stream) : kp_launch<128>(q, scales, out, map, a, stream);
+    const cudaError_t e = a.P == 8 ? (D == 64 ? kp_launch<64, 8>(q, scales, out, map, a, stream) : kp_launch<128, 8>(q, scales, out, map, a, stream))
+                                   : (D == 64 ? kp_launch<64, 16>(q, scales, out, map, a, stream) : kp_launch<128, 16>(q, scales, out, map, a, stream));
     if (e != cudaSuccess) {
         tk_set_error("attn_kv8: launch failed: %s", cudaGetErrorString(e));
         cudaGetLastError();

@@ -91,8 +91,9 @@ __device__ __forceinline__ void sync_128() { asm volatile("bar.sync 2, 128;" :::
 template <int D>
 constexpr int k8t_stages = 3;
 
-template <int D, int NR>
+template <int D, int NR, int KG>
 struct K8tSmem {
+    static constexpr int GROUPS = K8T_KEYS / KG;                                   // that share scales: 16 keys, or 8 where a page has no more
     static constexpr int STAGES = k8t_stages<D>;
     static constexpr int S_COLS = 2 * NR < 16 ? 16 : 2 * NR;                       // scores' columns: term, head
     static constexpr int O_COLS = 4 * NR < 16 ? 16 : 4 * NR;                       // outputs' columns: term, head
@@ -102,8 +103,8 @@ struct K8tSmem {
     static constexpr int KV = Q + (S_COLS * D < 1024 ? 1024 : S_COLS * D);         // stages: K tile, V tile
     static constexpr int STAGE = 2 * K8T_KEYS * D;
     static constexpr int BARS = KV + STAGES * STAGE;
-    static constexpr int SCALES = BARS + (2 * STAGES + 6) * 8 + 16;                // of a tile's eight groups of 16 keys: (key's, value's)
-    static constexpr int MISC = SCALES + STAGES * 8 * 8;
+    static constexpr int SCALES = BARS + (2 * STAGES + 6) * 8 + 16;                // of a tile's groups of keys: (key's, value's)
+    static constexpr int MISC = SCALES + STAGES * GROUPS * 8;
     static constexpr int BYTES = MISC + (16 * 4 + 4 * 16 * 4);                     // row factors, warps' maxima or sums
     static_assert(SCALES % 8 == 0 && MISC % 8 == 0, "pairs");
     // a share of the keys, for the CTAs that join theirs: [head][d] and the heads' maxima and sums, where the first tiles were
@@ -118,10 +119,11 @@ __device__ __forceinline__ uint64_t desc_keys16(uint32_t at) {
 }
 
 // D: head size; NR: query heads a KV head has, rounded up to 2, 4, 8 or 16
-template <int D, int NR>
+template <int D, int NR, int KG>
 __global__ void __launch_bounds__(K8T_THREADS, D == 64 && NR <= 4 ? 4 : 2)
 attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* out, const __grid_constant__ CUtensorMap map, const K8Args a) {
-    using L = K8tSmem<D, NR>;
+    using L = K8tSmem<D, NR, KG>;
+    constexpr int GROUPS = L::GROUPS, AHEAD = 32 / GROUPS;                         // tiles whose pages and scales a copying warp's lanes know
     constexpr int STAGES = L::STAGES;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     pdl_launch_dependents();
@@ -227,15 +229,15 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
     const uint32_t tmem_o = tmem + 64;
 
     if (warp >= 4 && warp < K8T_MMA_WARP) {
-        // ---- K and V: lane i knows the page and the scales of 16 positions of one of four tiles, and brings the page (or 128 positions of it)
+        // ---- K and V: lane i knows the page and the scales of KG positions of one of four tiles (KG = 8: two), and brings the page (or 128 positions of it)
         // if they are its first of the tile: keys one warp, values the other. (A warp's loads go out one after the other, 65 to 100 cycles
-        // each however they are issued: one warp for a tile's 16 set the pace at 1,450 cycles a tile.) The pages of four tiles are asked for
-        // eight tiles ahead, their scales four: no trip is waited for. ----
+        // each however they are issued: one warp for a tile's 16 set the pace at 1,450 cycles a tile.) The pages of four (two) tiles are asked for
+        // eight (four) tiles ahead, their scales half as many: no trip is waited for. ----
         const int which = warp - 4, per = 1 << min(a.p_shift, 7);
-        const int group = lane & 7, at_row = (group * 16) & (per - 1);        // (of a page, as far as a tile reaches)
+        const int group = lane & (GROUPS - 1), at_row = (group * KG) & (per - 1);        // (of a page, as far as a tile reaches)
         bool ok = true;
-        auto page_of = [&](int four) {
-            const int it = four * 4 + (lane >> 3), j = (t_begin + it) * K8T_KEYS + group * 16 - at_row;
+        auto page_of = [&](int block) {
+            const int it = block * AHEAD + lane / GROUPS, j = (t_begin + it) * K8T_KEYS + group * KG - at_row;
             return it < n_tiles && j <= pos && j + per > lo ? TK_PAGE(TK_K_KV8_ATTN, bt[j >> a.p_shift]) : -1;
         };
         auto scales_of = [&](int pg) {
@@ -247,22 +249,22 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
         float2* sc = reinterpret_cast<float2*>(smem_raw + L::SCALES);
         for (int it = 0; it < n_tiles; ++it) {
             const int s = it % STAGES;
-            if ((it & 3) == 0) {
+            if (it % AHEAD == 0) {
                 page = page_next;
                 scale = scale_next;
                 page_next = page_after;
                 scale_next = scales_of(page_next);
-                page_after = page_of(it / 4 + 2);
+                page_after = page_of(it / AHEAD + 2);
             }
             if (it >= STAGES) ok = k8_wait(kv_empty(s), (uint32_t)((it / STAGES - 1) & 1));
             if (!__all_sync(0xffffffffu, ok)) break;
-            const bool ours = (lane >> 3) == (it & 3), mine = ours && page >= 0 && at_row == 0;
+            const bool ours = lane / GROUPS == it % AHEAD, mine = ours && page >= 0 && at_row == 0;
             const int loads = __popc(__ballot_sync(0xffffffffu, mine));
             if (mine) {
-                const int row = ((page * 2 + which) * a.Hkv + kvh) * P + (((t_begin + it) * K8T_KEYS + group * 16) & (P - 1));
-                tma_load_2d(base + L::KV + (uint32_t)s * L::STAGE + (uint32_t)((which * K8T_KEYS + group * 16) * D), &map, 0, row, kv_full(s));
+                const int row = ((page * 2 + which) * a.Hkv + kvh) * P + (((t_begin + it) * K8T_KEYS + group * KG) & (P - 1));
+                tma_load_2d(base + L::KV + (uint32_t)s * L::STAGE + (uint32_t)((which * K8T_KEYS + group * KG) * D), &map, 0, row, kv_full(s));
             }
-            if (which == 0 && ours) sc[s * 8 + group] = scale;
+            if (which == 0 && ours) sc[s * GROUPS + group] = scale;
             __syncwarp();
             // (the phase ends with this arrival and the bytes, whichever come last)
             if (lane == 0) mbar_expect_tx(kv_full(s), (uint32_t)(loads * per * D));
@@ -323,7 +325,7 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
             // (after a failed wait the loop runs to its end without waiting: every thread meets every barrier)
             if (ok) ok = k8_wait(s_full(b), (uint32_t)(turn & 1)) && k8_wait(kv_full(it % STAGES), (uint32_t)((it / STAGES) & 1));
             ok = __all_sync(0xffffffffu, ok);
-            const float2 sc = reinterpret_cast<const float2*>(smem_raw + L::SCALES)[(it % STAGES) * 8 + (tid >> 4)];
+            const float2 sc = reinterpret_cast<const float2*>(smem_raw + L::SCALES)[(it % STAGES) * GROUPS + tid / KG];
             const int bits = __float_as_int(sc.y);
             const float ev = __int_as_float(0x4b000000 | (bits >> 23)) - 8388735.0f, inv_v = __int_as_float((254 << 23) - bits);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -480,11 +482,11 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
     }
 }
 
-template <int D, int NR>
+template <int D, int NR, int KG>
 cudaError_t k8t_launch(const void* q, const float* scales, void* out, const CUtensorMap& map, const K8Args& a, cudaStream_t stream) {
-    constexpr int smem = K8tSmem<D, NR>::BYTES;
+    constexpr int smem = K8tSmem<D, NR, KG>::BYTES;
     static std::atomic<uint64_t> done{0};
-    const cudaError_t e = k8_allow(attn_kv8_tc_kernel<D, NR>, smem, true, done);
+    const cudaError_t e = k8_allow(attn_kv8_tc_kernel<D, NR, KG>, smem, true, done);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.items * a.Hkv * a.nsplit));
@@ -494,26 +496,27 @@ cudaError_t k8t_launch(const void* q, const float* scales, void* out, const CUte
     cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
     cfg.numAttrs = k8_attributes(attr, a.nsplit);
-    return cudaLaunchKernelEx(&cfg, attn_kv8_tc_kernel<D, NR>, (const __nv_bfloat16*)q, scales, (__nv_bfloat16*)out, map, a);
+    return cudaLaunchKernelEx(&cfg, attn_kv8_tc_kernel<D, NR, KG>, (const __nv_bfloat16*)q, scales, (__nv_bfloat16*)out, map, a);
 }
 
-template <int D>
+template <int D, int KG>
 cudaError_t k8t_rows(const void* q, const float* scales, void* out, const CUtensorMap& map, const K8Args& a, cudaStream_t stream) {
     const int G = a.H / a.Hkv;
-    return G <= 2   ? k8t_launch<D, 2>(q, scales, out, map, a, stream)
-           : G <= 4 ? k8t_launch<D, 4>(q, scales, out, map, a, stream)
-           : G <= 8 ? k8t_launch<D, 8>(q, scales, out, map, a, stream)
-                    : k8t_launch<D, 16>(q, scales, out, map, a, stream);
+    return G <= 2   ? k8t_launch<D, 2, KG>(q, scales, out, map, a, stream)
+           : G <= 4 ? k8t_launch<D, 4, KG>(q, scales, out, map, a, stream)
+           : G <= 8 ? k8t_launch<D, 8, KG>(q, scales, out, map, a, stream)
+                    : k8t_launch<D, 16, KG>(q, scales, out, map, a, stream);
 }
 
 }  // namespace
 
-// The arguments of tk_attn_kv8 for single tokens (attention_kv8.cu checks them): bfloat16, pages that are a power of two and 16 or more.
+// The arguments of tk_attn_kv8 for single tokens (attention_kv8.cu checks them): bfloat16, pages that are a power of two and 8 or more.
 int tk_attn_kv8_tc(const void* q, const void* pool, const float* scales, void* out, const void* args, int D, cudaStream_t stream) {
     const K8Args& a = *static_cast<const K8Args*>(args);
     CUtensorMap map = {};
     TK_CHECK_ARG(k8_map(&map, pool, D, a.P < K8T_KEYS ? a.P : K8T_KEYS), "attn_kv8: cuTensorMapEncodeTiled failed");
-    const cudaError_t e = D == 64 ? k8t_rows<64>(q, scales, out, map, a, stream) : k8t_rows<128>(q, scales, out, map, a, stream);
+    const cudaError_t e = a.P == 8 ? (D == 64 ? k8t_rows<64, 8>(q, scales, out, map, a, stream) : k8t_rows<128, 8>(q, scales, out, map, a, stream))
+                                   : (D == 64 ? k8t_rows<64, 16>(q, scales, out, map, a, stream) : k8t_rows<128, 16>(q, scales, out, map, a, stream));
     if (e != cudaSuccess) {
         tk_set_error("attn_kv8: launch failed: %s", cudaGetErrorString(e));
         cudaGetLastError();

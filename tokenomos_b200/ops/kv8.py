@@ -130,8 +130,8 @@ def _attend(q, pool, scales, out, positions, tok_seq, block_table, tok0, ntok, i
 
 
 def _whole_pages(P: int) -> bool:
-    """Whether pages are a power of two and 16 positions or more, as the tcgen05 kernels take them."""
-    return P >= 16 and not P & (P - 1)
+    """Whether pages are a power of two and 8 positions or more, as the tcgen05 kernels take them."""
+    return P >= 8 and not P & (P - 1)
 
 
 def attention_kv8_decode(q: torch.Tensor, pool: torch.Tensor, scales: torch.Tensor, out: torch.Tensor, positions: torch.Tensor,
