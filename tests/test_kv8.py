@@ -401,10 +401,11 @@ def test_attention_of_portions_and_single_tokens_in_one_step(dtype, H, G, D, P):
 @pytest.mark.parametrize("window", [None, 7, 8, 100, -24])
 @pytest.mark.parametrize("H, G, D, P", [(4, 2, 64, 8), (3, 1, 64, 8), (32, 8, 128, 8), (14, 2, 64, 8), (16, 1, 128, 8), (6, 2, 64, 16), (5, 1, 128, 32), (22, 2, 64, 16),
                                         (39, 3, 64, 64), (7, 1, 64, 8)])
-def test_attention_over_pages_of_8_and_of_groups_that_do_not_divide_a_tile(H, G, D, P, window):
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attention_over_pages_of_8_and_of_groups_that_do_not_divide_a_tile(dtype, H, G, D, P, window):
     lens = [1, 8, 9, 63, 64, 65, 257, 1500, 130, 700, 2300]
     new = [1, 8, 2, 63, 1, 40, 200, 1, 129, 700, 45]
-    check_attention(Cache(lens, G, D, P, seed=P).fill(seed=H, spread=4), new, H, torch.bfloat16, window=window)
+    check_attention(Cache(lens, G, D, P, seed=P).fill(seed=H, spread=4), new, H, dtype, window=window)
 
 
 @gpu

@@ -1,5 +1,5 @@
-// Attention over the 8-bit cache (kv8.cuh) on mma.sync.m16n8k16, with float16 operands and 32-bit sums: single tokens of any
-// model, and prompt portions of the sizes that the tcgen05 kernel (attention_kv8_tc.cu) does not take.
+// Attention over the 8-bit cache (kv8.cuh) on mma.sync.m16n8k16, with float16 operands and 32-bit sums: all of the 32-bit
+// models, and pages that the tcgen05 kernels (attention_kv8_tc.cu, attention_kv8_prefill.cu) do not take.
 //
 //   o[r] = sum_j p_rj v_j / sum_j p_rj,   p_rj = exp(scale * q_r . k_j),   k_j = s_K kb_j,  v_j = s_V vb_j   (bytes kb, vb)
 //
@@ -7,7 +7,7 @@
 // keys; its warps walk groups of 32 (16 for heads of 128) keys in turn and are joined through shared memory, the CTAs of a
 // row through scratch memory and a second kernel.
 //
-// Pages of 16 positions and more come by bulk copies, up to three units of 32 keys (heads of 128: 16) a warp in shared memory or on their way; smaller or odd ones are read by
+// Pages of a power of two of 8 positions and more come by bulk copies (32-bit), up to three units of 32 keys (heads of 128: 16) a warp in shared memory or on their way; smaller or odd ones are read by
 // each lane. From bytes to operands nothing is moved between lanes: the order of a product's inner index is free as long as both operands follow it, and the order of the output's columns is
 // too: a lane reads D / 4 bytes side by side of one key's row (16 bytes for D = 64; four lanes a row) and uses them as its fragments of all the D / 16
 // steps of q . k, with q's fragments laid out to match; and of a value row it reads D / 8 bytes, one for each of the D / 8 column tiles, so that two rows' bytes
@@ -52,10 +52,10 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-// T: type of q and the output. D: head size. PAGE16: pages are a multiple of 16 positions and a power of two, so 16 keys that begin at a multiple of
-// 16 lie in one page; otherwise every lane looks its own keys' pages up.
-template <typename T, int D, bool PAGE16>
-__global__ void __launch_bounds__(K8_THREADS, D == 64 && PAGE16 ? (sizeof(T) == 2 ? 4 : 3) : 2)
+// T: type of q and the output. D: head size. KG: 16 where pages are a power of two of 16 positions or more, so 16 keys that begin at a multiple of 16 lie in
+// one page, 8 for pages of 8; 0: every lane looks its own keys' pages up.
+template <typename T, int D, int KG>
+__global__ void __launch_bounds__(K8_THREADS, D == 64 && KG > 0 ? 3 : 2)
 attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, const K8Args a) {
     constexpr bool WIDE = sizeof(T) == 4;                // q and the weights as two float16
     constexpr int U = D == 64 ? 2 : 1;                   // groups of 16 keys a warp takes at a time
@@ -63,6 +63,8 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
     constexpr int KW = D / 64;                           // 16-byte words a lane reads of a key
     constexpr int VW = D / 32;                           // 4-byte words a lane reads of a value row
     constexpr int UNIT = U * 32 * D;                     // a unit's bytes
+    constexpr bool BULK = KG > 0;
+    constexpr int HALVES = KG == 8 ? 2 : 1, PIECES = U * HALVES;      // pages' pieces (of KG keys) of a group, of a unit
     extern __shared__ __align__(128) float smem[];
     pdl_launch_dependents();
     pdl_wait();
@@ -131,13 +133,15 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
     const int units = (g_end - g_begin + U - 1) / U;
     const int mine = units > warp ? (units - warp + K8_WARPS - 1) / K8_WARPS : 0;         // this warp's: unit warp, warp + K8_WARPS, ...
     auto group_of = [&](int k, int u) { return g_begin + (warp + k * K8_WARPS) * U + u; };
-    // PAGE16: lane i knows the page and, from when its bytes are asked for, the scales of group i of a block of 32 groups
-    constexpr int BLOCK = 32 / U;
+    // lane i knows the page and, from when its bytes are asked for, the scales of piece i of a block of 32 pieces
+    constexpr int BLOCK = 32 / PIECES;
     int page_now = 0, page_then = 0;
     float sk_now = 1.f, sv_now = 1.f, sk_then = 1.f, sv_then = 1.f;
+    const int p_end = BULK ? min(g_end * HALVES, pos_last / (BULK ? KG : 16) + 1) : 0;       // (the last group's second page may not be there)
+    auto piece_of = [&](int k, int i) { return group_of(k, 0) * HALVES + i; };
     auto page_of_block = [&](int block) {
-        const int gr = group_of(block * BLOCK + lane / U, lane % U);
-        return gr < g_end ? TK_PAGE(TK_K_KV8_ATTN, bt[(gr << 4) >> a.p_shift]) : -1;
+        const int pc = piece_of(block * BLOCK + lane / PIECES, lane % PIECES);
+        return pc < p_end ? TK_PAGE(TK_K_KV8_ATTN, bt[(pc * KG) >> a.p_shift]) : -1;
     };
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + (uint32_t)warp * (K8_DEPTH * UNIT);
     const uint32_t bars = (uint32_t)__cvta_generic_to_shared(smem) + K8_WARPS * K8_DEPTH * UNIT + (uint32_t)warp * (K8_DEPTH * 8);
@@ -151,22 +155,22 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
             sk_then = page_now >= 0 ? sc[0] : 1.f;
             sv_then = page_now >= 0 ? sc[a.Hkv] : 1.f;
         }
-        const int first = group_of(k, 0), n = min(U, g_end - first);
+        const int first = piece_of(k, 0), n = min(PIECES, p_end - first);
         const uint32_t bar = bars + (uint32_t)(k % K8_DEPTH) * 8;
-        const int page = __shfl_sync(0xffffffffu, page_now, (k % BLOCK) * U + (lane >> 1) % U);
+        const int page = __shfl_sync(0xffffffffu, page_now, (k % BLOCK) * PIECES + (lane >> 1) % PIECES);
         if (lane == 0)
-            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n * 32 * D) : "memory");
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n * 2 * KG * D) : "memory");
         __syncwarp();
         if (lane < 2 * n) {
-            const int u = lane >> 1, which = lane & 1;
-            const uint8_t* src = head + (size_t)page * page_bytes + which * v_delta + (uint32_t)((((first + u) << 4) & (P - 1)) * D);
+            const int i = lane >> 1, which = lane & 1;
+            const uint8_t* src = head + (size_t)page * page_bytes + which * v_delta + (uint32_t)((((first + i) * KG) & (P - 1)) * D);
             asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                             ring + (uint32_t)(k % K8_DEPTH) * UNIT + (uint32_t)(u * 32 * D + which * 16 * D)),
-                         "l"(src), "r"(16 * D), "r"(bar)
+                             ring + (uint32_t)(k % K8_DEPTH) * UNIT + (uint32_t)(i / HALVES * 32 * D + which * 16 * D + i % HALVES * KG * D)),
+                         "l"(src), "r"(KG * D), "r"(bar)
                          : "memory");
         }
     };
-    if constexpr (PAGE16) {
+    if constexpr (BULK) {
         if (lane == 0) {
             for (int i = 0; i < K8_DEPTH; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bars + i * 8) : "memory");
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -192,10 +196,11 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
         const int gr = group_of(k, 0);
         const bool inner = (gr << 4) >= lo && ((gr + U) << 4) <= min(pos_last + 1, g_end << 4);      // all of its keys are read
         const uint8_t* here = stage + (k % K8_DEPTH) * UNIT;
-        constexpr int NS = PAGE16 ? 1 : 4;               // scales a group has for a lane: one, or one for each of its four keys
+        constexpr int NS = BULK ? HALVES : 4;            // scales a group has for a lane: one, two (its tiles'), or one for each of its four keys
+        auto scale_at = [](int t, int e) { return NS == 1 ? 0 : NS == 2 ? t : 2 * t + e; };
         float ksc[U][NS], vsc[U][NS];
         uint4 kw[U][2][KW];
-        if constexpr (PAGE16) {
+        if constexpr (BULK) {
             issue(k + K8_DEPTH - 1);
             if (k % BLOCK == 0) {                        // (asked for when the first of the block's bytes were)
                 sk_now = sk_then;
@@ -254,9 +259,12 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
                     if constexpr (WIDE) mma_f16(x[u][t], qb[ks], b0, b1);
                 }
             }
-            if constexpr (PAGE16) {
-                ksc[u][0] = __shfl_sync(0xffffffffu, sk_now, (k % BLOCK) * U + u);
-                vsc[u][0] = __shfl_sync(0xffffffffu, sv_now, (k % BLOCK) * U + u);
+            if constexpr (BULK) {
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
+                    ksc[u][i] = __shfl_sync(0xffffffffu, sk_now, (k % BLOCK) * PIECES + u * HALVES + i);
+                    vsc[u][i] = __shfl_sync(0xffffffffu, sv_now, (k % BLOCK) * PIECES + u * HALVES + i);
+                }
             }
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
@@ -280,12 +288,13 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
             }
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                if constexpr (PAGE16) {
+                if constexpr (NS == 1) {
                     const float most = fmaxf(fmaxf(x[u][0][2 * r], x[u][0][2 * r + 1]), fmaxf(x[u][1][2 * r], x[u][1][2 * r + 1]));
                     top[r] = fmaxf(top[r], fmaf(most, kc[u][0][r], ev[u][0]));
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) top[r] = fmaxf(top[r], fmaf(x[u][i >> 1][2 * r + (i & 1)], kc[u][i][r], ev[u][i]));
+                    for (int i = 0; i < 4; ++i)
+                        top[r] = fmaxf(top[r], fmaf(x[u][i >> 1][2 * r + (i & 1)], kc[u][scale_at(i >> 1, i & 1)][r], ev[u][scale_at(i >> 1, i & 1)]));
                 }
             }
         }
@@ -313,7 +322,7 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int hrow = 0; hrow < 2; ++hrow) {
-                    const int i0 = PAGE16 ? 0 : 2 * t, i1 = PAGE16 ? 0 : 2 * t + 1;
+                    const int i0 = scale_at(t, 0), i1 = scale_at(t, 1);
                     const float w0 = k8_exp2(fmaf(x[u][t][2 * hrow], kc[u][i0][hrow], ev[u][i0] + base[hrow]));
                     const float w1 = k8_exp2(fmaf(x[u][t][2 * hrow + 1], kc[u][i1][hrow], ev[u][i1] + base[hrow]));
                     l[hrow] = fmaf(w0, inv_vs[u][i0], l[hrow]);
@@ -330,7 +339,7 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
                 const int row = key_in_group(i >> 1, i & 1), j = ((gr + u) << 4) + row;
                 const bool there = inner || (gr + u < g_end && j >= lo && j <= pos_last);
                 const uint8_t* src = here + u * 32 * D + 16 * D + row * D + g * (D / 8);
-                if constexpr (!PAGE16)
+                if constexpr (!BULK)
                     if (there) src = head + (size_t)TK_PAGE(TK_K_KV8_ATTN, bt[j / P]) * page_bytes + v_delta + (size_t)(j % P) * D + g * (D / 8);
                 // (what is not to be read is in shared memory all the same where a page's bytes came as one, and never matters)
                 if constexpr (VW == 2) {
@@ -414,25 +423,33 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
     }
 }
 
-template <typename T, int D, bool PAGE16>
+template <typename T, int D, int KG>
 cudaError_t k8_launch(const void* q, const void* pool, const float* scales, void* out, const K8Args& a, cudaStream_t stream) {
     constexpr int shares = (K8_WARPS * K8_ROWS * (D + 4) + 2 * K8_WARPS * K8_ROWS) * 4;
-    constexpr int ring = PAGE16 ? K8_WARPS * K8_DEPTH * (4096 + 8) : 0;
+    constexpr int ring = KG > 0 ? K8_WARPS * K8_DEPTH * (4096 + 8) : 0;
     constexpr int smem = ring > shares ? ring : shares;
     if (smem > 48 * 1024) {
         static std::atomic<uint64_t> done{0};
-        const cudaError_t e = k8_allow(attn_kv8_kernel<T, D, PAGE16>, smem, false, done);
+        const cudaError_t e = k8_allow(attn_kv8_kernel<T, D, KG>, smem, false, done);
         if (e != cudaSuccess) return e;
     }
-    return tk_launch(attn_kv8_kernel<T, D, PAGE16>, dim3((unsigned)(a.items * a.Hkv * a.nsplit)), dim3(K8_THREADS), smem, stream, (const T*)q,
+    return tk_launch(attn_kv8_kernel<T, D, KG>, dim3((unsigned)(a.items * a.Hkv * a.nsplit)), dim3(K8_THREADS), smem, stream, (const T*)q,
                      (const uint8_t*)pool, scales, (T*)out, a);
+}
+
+// (bfloat16 comes here for pages that the tcgen05 kernels do not take)
+template <typename T, int D>
+cudaError_t k8_pages(const void* q, const void* pool, const float* scales, void* out, const K8Args& a, cudaStream_t stream) {
+    if constexpr (sizeof(T) == 4) {
+        if (a.p_shift >= 4) return k8_launch<T, D, 16>(q, pool, scales, out, a, stream);
+        if (a.p_shift == 3) return k8_launch<T, D, 8>(q, pool, scales, out, a, stream);
+    }
+    return k8_launch<T, D, 0>(q, pool, scales, out, a, stream);
 }
 
 template <typename T>
 cudaError_t k8_dispatch(const void* q, const void* pool, const float* scales, void* out, const K8Args& a, int D, cudaStream_t stream) {
-    const bool page16 = a.p_shift >= 4;
-    cudaError_t e = D == 64 ? (page16 ? k8_launch<T, 64, true>(q, pool, scales, out, a, stream) : k8_launch<T, 64, false>(q, pool, scales, out, a, stream))
-                            : (page16 ? k8_launch<T, 128, true>(q, pool, scales, out, a, stream) : k8_launch<T, 128, false>(q, pool, scales, out, a, stream));
+    const cudaError_t e = D == 64 ? k8_pages<T, 64>(q, pool, scales, out, a, stream) : k8_pages<T, 128>(q, pool, scales, out, a, stream);
     if (e != cudaSuccess || a.nsplit == 1) return e;
     const unsigned grid = (unsigned)(((int64_t)a.items * a.Hkv * a.rows_most + 3) / 4);
     return D == 64 ? tk_launch(attn_kv8_merge_kernel<T, 64>, dim3(grid), dim3(128), 0, stream, (T*)out, a, K8_LIFT)
