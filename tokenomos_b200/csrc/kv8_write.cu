@@ -161,7 +161,15 @@ qk_norm_rope_write8_kernel(const T* qkv, int64_t qkv_stride, T* q_out, uint8_t* 
     const int sub = lane / LPH, c = (lane % LPH) * 8, half = a.R >> 1;
     const bool queries = (int)blockIdx.x >= a.kv_blocks, norm = wq != nullptr;
     float w[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
-    if (norm) load8((queries ? wq : wk) + c, w);         // (nobody writes them: asked for while the kernel before ends)
+    if (norm) {                                          // (nobody writes them: asked for while the kernel before ends)
+        const float* from = (queries ? wq : wk) + c;
+        if ((reinterpret_cast<uintptr_t>(from) & 15) == 0) {
+            load8(from, w);
+        } else {                                         // (a vector of floats may begin at any of them)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = from[e];
+        }
+    }
     const float f_mine = tid % HALF < half ? freq[tid % HALF] : 0.f;
     pdl_wait();
     // the angles of `count` tokens, a frequency a thread
@@ -320,7 +328,7 @@ qk_norm_rope_write8_kernel(const T* qkv, int64_t qkv_stride, T* q_out, uint8_t* 
 }  // namespace
 
 // qkv: [T, (H + 2 Hkv) D] with row stride `qkv_stride`, 16-byte aligned rows; pool: [pages, 2, Hkv, P, D] bytes, scales: [pages, 2, Hkv]. wq / wk:
-// both or neither. freq: [R / 2]. The tokens of a sequence lie side by side in the step, at consecutive positions.
+// both or neither, D floats at any float's address. freq: [R / 2]. The tokens of a sequence lie side by side in the step, at consecutive positions.
 TK_API int tk_qk_norm_rope_write8(const void* qkv, int64_t qkv_stride, void* q_out, void* pool, float* scales, const float* wq,
                                   const float* wk, float eps, const float* freq, float cs_mult, int interleaved, const int* positions,
                                   const int* tok_seq, const int* block_table, int bt_stride, int T_, int H, int Hkv, int D, int R, int P,
