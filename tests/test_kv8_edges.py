@@ -3,10 +3,14 @@ their range, weights that are small beside their row's largest."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
-from test_kv8 import Cache, write
+from test_kv8 import Cache, i32, run_attention, write
+from tokenomos_b200 import ops
+from tokenomos_b200.ops import _lib
 
 gpu = pytest.mark.gpu
 
@@ -33,3 +37,77 @@ def test_norm_weights_may_begin_at_any_float(D, T, dtype):
         q2, _ = write(got, [(0, 0, x)], H, wq, wk, 1e-6, freq)
         assert torch.equal(q, q2) and torch.equal(got.scales.view(torch.int32), want.scales.view(torch.int32))
         assert torch.equal(got.pool.view(torch.uint8), want.pool.view(torch.uint8))
+
+
+# ---- weights that are small beside their row's largest ----
+
+def rows_with_one_large_weight(n, H, G, D, P, share, T, seed=0):
+    """A sequence of n positions whose first key takes `share` of every row's weight and has values of 0; the others' weights are log-normal, their
+    values random. (cache, q [T, H, D], scale): all that q asks of a key are its first two elements, which both terms of q hold exactly."""
+    gen = torch.Generator().manual_seed(seed)
+    cache = Cache([n], G, D, P, seed=seed)
+    pages = cache.table[0].long().cuda()
+    kv = (torch.randn(len(pages), 2, G, P, D, generator=gen) * 60).to(torch.float8_e4m3fn)
+    score = torch.randn(len(pages), G, P, generator=gen)
+    kv.view(torch.uint8)[:, 0, :, :, 0] = (score * 64).to(torch.float8_e4m3fn).view(torch.uint8)
+    kv.view(torch.uint8)[:, 0, :, :, 1] = 0
+    kv.view(torch.uint8)[0, :, :, 0, :2] = 0
+    kv.view(torch.uint8)[0, 1, :, 0] = 0
+    kv[0, 0, :, 0, 1] = torch.tensor(256.0).to(torch.float8_e4m3fn)
+    cache.pool.view(torch.uint8)[pages] = kv.view(torch.uint8).cuda()
+    cache.scales[pages] = 2.0 ** -6
+    first = math.log(share / (1 - share) * n * math.exp(0.5))               # (the mean of a log-normal number is e^(1/2))
+    q = torch.zeros(T, H, D)
+    q[..., 0], q[..., 1] = 1.0, first / 4
+    return cache, q.to(torch.bfloat16).cuda(), 1.0
+
+
+@gpu
+@pytest.mark.parametrize("share", [0.5, 0.99, 0.999])
+@pytest.mark.parametrize("n, H, G, D, P, T", [(3000, 32, 8, 64, 16, 64), (3000, 8, 8, 64, 8, 64), (2000, 64, 8, 64, 16, 40), (3000, 128, 8, 128, 16, 38), (2500, 16, 8, 128, 32, 64),
+                                              (32000, 8, 2, 64, 16, 2), (32000, 4, 1, 128, 16, 1)])
+def test_small_weights_beside_a_large_one_keep_their_bits(n, H, G, D, P, T, share):
+    """Single tokens, unshared (T G CTAs and more fill the GPU) and shared out. The errors are independent of each other: the output's rounding (half a
+    step, 2^-8 of an element), each weight's to float16's eleven bits (2^-11 of it) or to half of float16's smallest step, 2^-25 beside a largest
+    weight of 2^6 at least; uniform ones, whose root mean square is their largest over sqrt(3). A quarter is left for the samples, 64 elements a
+    row and more. (With q's two elements and powers of two as scales, scores are exact to 32-bit rounding: 2^-21 of a weight.)"""
+    cache, q, scale = rows_with_one_large_weight(n, H, G, D, P, share, T)
+    if n < 4000:
+        assert _lib.call("tk_attn_kv8_splits", T, H, G, D, n, n, 148, 1) == 1
+    pos, seq = i32([n - 1] * T), i32([0] * T)
+    out = torch.full_like(q, 7.0)
+    ops.attention_kv8_decode(q, cache.pool, cache.scales, out, pos, seq, cache.table_dev, None, None, scale, n)
+    k, v = cache.of(0)
+    p = torch.softmax(torch.einsum("hd,gnd->hgn", q[0, :1].double(), k)[0] * scale, -1)          # [G, n]
+    assert ((p[:, 0] - share).abs() <= 0.15 * (1 - share)).all()
+    want = torch.einsum("gn,gnd->gd", p, v)
+    fine = torch.einsum("gn,gnd->gd", p.square(), v.square())
+    coarse = p[:, :1].square() * v.square().sum(1)
+    mean = (want.square() * 2.0 ** -16 + fine * 2.0 ** -22 + coarse * 2.0 ** -62).sum() / 3
+    got = out.double().view(T, G, H // G, D)
+    for t in range(T):
+        for r in range(H // G):
+            off = (got[t, :, r] - want).norm()
+            assert off <= 1.25 * mean.sqrt(), (t, r, (off / want.norm()).item(), (mean.sqrt() / want.norm()).item())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("share", [0.5, 0.999])
+def test_a_prompts_last_row_and_the_same_token_decoded_agree(share, dtype):
+    """A row of a portion and the same row as a single token: both within the bound above of the definition, so within twice it of each other. A 32-bit
+    weight is off by its score's roundings: four of numbers of up to 40, as logarithms of 2 (2^-17 of the weight)."""
+    n, H, G, D = 3000, 8, 2, 64
+    cache, q, scale = rows_with_one_large_weight(n, H, G, D, 16, share, 40, seed=1)
+    q = q.to(dtype)
+    outs = [run_attention(cache, q[:new], [new], None, scale)[0][-1].double().view(G, H // G, D) for new in (1, 40)]
+    k, v = cache.of(0)
+    p = torch.softmax(torch.einsum("hd,gnd->hgn", q[0, :1].double(), k)[0] * scale, -1)
+    want = torch.einsum("gn,gnd->gd", p, v)
+    fine = torch.einsum("gn,gnd->gd", p.square(), v.square())
+    coarse = p[:, :1].square() * v.square().sum(1)
+    unit, each = torch.finfo(dtype).eps / 2, 2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -17
+    mean = (want.square() * (unit ** 2 + each ** 2) + fine * each ** 2 + coarse * 2.0 ** -62).sum() / 3
+    for out in outs:
+        for r in range(H // G):
+            assert (out[:, r] - want).norm() <= 1.25 * mean.sqrt()

@@ -6,10 +6,12 @@
 //
 // What is not 8-bit is a sum of 8-bit terms, a column each, added up when they are read: e4m3 has four significant bits, so q (after
 // division by a power of two that brings its row's largest to [128, 256)) is two terms, exactly for elements down to 2^-12 of the row's
-// largest and to 2^-18 of that below. A weight is four: two that leave 2^-8 of it or 2^-10 (e4m3's smallest steps), and two of what they leave times
-// 2^8. The weights' reference maximum follows lazily (raised when a row exceeds it by 2^2) and weights are lifted by 2^6 (at most 256, of 448): a
-// weight (rounded to float16 first, so that the terms are packed arithmetic) is off by at most 2^-11 of itself or 2^-24 of the row's largest. (Two terms alone lose the many small weights beside a large one: 30,000
-// keys that share half of a row's weight with one that has the other half would be off by a tenth.) A value block's scale is in the
+// largest and to 2^-18 of that below. A weight is rounded to float16 and is four terms, each the e4m3 of what those before it leave times 2^5: of a weight of at
+// most 2^8 a term leaves at most 2^3, so 2^8 again goes into the next one, and the last one's smallest step, 2^-9 2^-15, is float16's: the four are the
+// float16 weight exactly. The weights' reference maximum follows lazily (raised when a row exceeds it by 2^2) and weights are lifted by 2^6 (at most 256, of
+// 448): a weight is off by at most 2^-11 of itself or, where that is more, by 2^-31 of the row's largest (half of float16's smallest step against 2^6), as in the form for portions. (Terms
+// of one size lose the many small weights beside a large one: with factors of 1, 1, 2^8 and 2^8, 3,000 keys that have a thousandth of a row's weight between
+// them, beside one that has the rest and a value of 0, came out 6 % off; now 0.2 %, the output's own rounding.) A value block's scale is in the
 // exponent, as in attention_kv8.cu. Columns cost nothing here: a product's time is that of reading its 128 x 32 or D x 32 bytes of the first operand
 // from shared memory. (With the heads as the M side of the second product, 32 rows of 128, and the terms one after the other, the products
 // alone took 575 cycles a tile of 128 keys, and 8 tokens behind 32,000 positions 71 us.)
@@ -45,7 +47,7 @@ constexpr int K8T_KEYS = 128;
 constexpr int K8T_COPIERS = 2;                             // warps that bring keys, and values
 constexpr int K8T_MMA_WARP = 4 + K8T_COPIERS, K8T_THREADS = (K8T_MMA_WARP + 1) * 32;
 constexpr int K8T_PTERMS = 4;
-constexpr float K8T_LAZY = 2.0f, K8T_LIFT = 6.0f, K8T_FINE = 256.0f;
+constexpr float K8T_LAZY = 2.0f, K8T_LIFT = 6.0f, K8T_FINER = 32.0f;       // (a term's factor over the one before)
 
 // eight columns of this thread's lane; the loads of several calls are waited for together
 __device__ __forceinline__ void tmem_ld8_start(uint32_t addr, uint32_t* r) {
@@ -391,15 +393,14 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
                     w[h] = k8_exp2(y[r + h]);
                     l[r + h] = fmaf(w[h], inv_v, l[r + h]);
                 }
-                __half2 left = __floats2half2_rn(w[0], w[1]);        // (what a term leaves of a float16 is one)
+                __half2 left = __floats2half2_rn(w[0], w[1]);        // (what a term leaves of a float16 is one, and so is 2^5 times that)
 #pragma unroll
                 for (int t = 0; t < K8T_PTERMS; ++t) {
                     uint16_t two;
                     asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(two) : "r"(*reinterpret_cast<const uint32_t*>(&left)));
                     terms[(t * NR + r) / 4] |= (uint32_t)two << (8 * ((t * NR + r) & 2));
                     const uint32_t back = e4m3x2_to_half2(two);
-                    left = __hsub2(left, *reinterpret_cast<const __half2*>(&back));
-                    if (t == 1) left = __hmul2(left, __float2half2_rn(K8T_FINE));
+                    left = __hmul2(__hsub2(left, *reinterpret_cast<const __half2*>(&back)), __float2half2_rn(K8T_FINER));
                 }
             }
             unsigned char* p = smem_raw + L::P + b * L::P_BYTES + tid * 16;
@@ -437,7 +438,9 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
                 if (r >= G) continue;
-                float o = fmaf(v[2 * NR + r] + v[3 * NR + r], 1.f / K8T_FINE, v[r] + v[NR + r]);
+                float o = v[3 * NR + r];
+#pragma unroll
+                for (int t = K8T_PTERMS - 2; t >= 0; --t) o = fmaf(o, 1.f / K8T_FINER, v[t * NR + r]);
                 float l_r = (by_warp[r] + by_warp[16 + r]) + (by_warp[32 + r] + by_warp[48 + r]);
                 const int head = kvh * G + r;
                 if (a.nsplit == 1) {
