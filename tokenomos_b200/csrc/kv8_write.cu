@@ -163,12 +163,8 @@ qk_norm_rope_write8_kernel(const T* qkv, int64_t qkv_stride, T* q_out, uint8_t* 
     float w[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
     if (norm) {                                          // (nobody writes them: asked for while the kernel before ends)
         const float* from = (queries ? wq : wk) + c;
-        if ((reinterpret_cast<uintptr_t>(from) & 15) == 0) {
-            load8(from, w);
-        } else {                                         // (a vector of floats may begin at any of them)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = from[e];
-        }
+        for (int e = 0; e < 8; ++e) w[e] = from[e];      // (a vector of floats may begin at any of them; 16 bytes at a time is no faster)
     }
     const float f_mine = tid % HALF < half ? freq[tid % HALF] : 0.f;
     pdl_wait();
