@@ -111,3 +111,35 @@ def test_a_prompts_last_row_and_the_same_token_decoded_agree(share, dtype):
     for out in outs:
         for r in range(H // G):
             assert (out[:, r] - want).norm() <= 1.25 * mean.sqrt()
+
+
+# ---- norms ----
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_head_whose_squares_overflow_is_zero_as_in_the_16_bit_write(D, dtype):
+    """Elements of 1e25: their squares' mean is infinite in 32 bits, what is divided by its root is 0, in the query, in the cached key, and in
+    ``qk_norm_rope_write``; the token is not marked. One infinite element makes NaN of the head and marks the token in its KV head."""
+    H, G, P = 2, 2, 16
+    g = torch.Generator().manual_seed(D)
+    x = torch.randn(4, H + 2 * G, D, generator=g)
+    x[1, :H + G] *= 1e25
+    x[2, 0, 5] = math.inf
+    x[2, H + 1, 7] = math.inf
+    x = x.to(dtype).cuda()
+    w = (torch.rand(2, D, generator=g) + 0.5).cuda()
+    freq = torch.exp(-torch.arange(D // 2) * 0.2).cuda()
+    cache = Cache([4], G, D, P)
+    q, pos = write(cache, [(0, 0, x.view(4, -1))], H, w[0].contiguous(), w[1].contiguous(), 1e-6, freq)
+    wide = torch.zeros(cache.pool.shape, dtype=dtype, device="cuda")
+    q16 = ops.qk_norm_rope_write(x.view(4, -1), wide, w[0].contiguous(), w[1].contiguous(), 1e-6, freq, pos, i32([0] * 4), cache.table_dev, H, G, D, P)
+    page = int(cache.table[0, 0])
+    assert (q16[1] == 0).all() and (wide[page, 0, :, 1] == 0).all()
+    assert (q[1] == 0).all() and (cache.of(0)[0, :, 1] == 0).all()
+    assert torch.isfinite(q[[0, 1, 3]].float()).all() and torch.isfinite(cache.of(0)[:, :, [0, 1, 3]]).all()
+    assert q[2, 0].isnan().any() and torch.isfinite(q[2, 1].float()).all()
+    assert cache.of(0)[0, 1, 2].isnan().all() and torch.isfinite(cache.of(0)[0, 0, 2]).all()
+    # (values are not normed)
+    v = x[1, H + G:].double()
+    assert ((cache.of(0)[1, :, 1] - v).abs() <= v.abs() / 16 + cache.value_scales(0)[:, 1:2] * 2.0 ** -10).all()

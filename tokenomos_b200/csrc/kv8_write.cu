@@ -92,7 +92,9 @@ __device__ __forceinline__ void norm_rotate(float (&x)[8], bool norm, const floa
         for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         const float mean = fmaf(ss, 1.0f / (LPH * 8), a.eps);
         float rstd = rsqrtf(mean);
-        rstd = rstd * fmaf(-0.5f * mean * rstd, rstd, 1.5f);         // (a Newton step: to the last bit or two)
+        // a Newton step: to the last bit or two. (Of an infinite mean the root's inverse is 0 and stays so: the step would make NaN of 0 x infinity, and
+        // mark a token whose elements are all finite)
+        if (rstd != 0.f) rstd = rstd * fmaf(-0.5f * mean * rstd, rstd, 1.5f);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = x[i] * rstd * w[i];
     }
