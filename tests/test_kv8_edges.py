@@ -8,12 +8,19 @@ import math
 import pytest
 import torch
 
-from test_kv8 import Cache, i32, run_attention, write
+from test_kv8 import Cache, attend, i32, run_attention, within, write
 from tokenomos_b200 import ops
 from tokenomos_b200.ops import _lib
 
 gpu = pytest.mark.gpu
 
+
+def shares_of_tokens(T, H, G, D, P, n):
+    """How many CTAs share each of T single tokens' keys in the tcgen05 form, behind n positions each."""
+    return _lib.lib().tk_attn_kv8_tc_splits(T, H, G, D, P, n, n)
+
+
+# ---- operands that lie where nobody expects them ----
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -73,7 +80,7 @@ def test_small_weights_beside_a_large_one_keep_their_bits(n, H, G, D, P, T, shar
     row and more. (With q's two elements and powers of two as scales, scores are exact to 32-bit rounding: 2^-21 of a weight.)"""
     cache, q, scale = rows_with_one_large_weight(n, H, G, D, P, share, T)
     if n < 4000:
-        assert _lib.call("tk_attn_kv8_splits", T, H, G, D, n, n, 148, 1) == 1
+        assert shares_of_tokens(T, H, G, D, P, n) == 1
     pos, seq = i32([n - 1] * T), i32([0] * T)
     out = torch.full_like(q, 7.0)
     ops.attention_kv8_decode(q, cache.pool, cache.scales, out, pos, seq, cache.table_dev, None, None, scale, n)
@@ -143,3 +150,50 @@ def test_a_head_whose_squares_overflow_is_zero_as_in_the_16_bit_write(D, dtype):
     # (values are not normed)
     v = x[1, H + G:].double()
     assert ((cache.of(0)[1, :, 1] - v).abs() <= v.abs() / 16 + cache.value_scales(0)[:, 1:2] * 2.0 ** -10).all()
+
+
+# ---- how many CTAs share a row's keys ----
+
+@gpu
+@pytest.mark.parametrize("P", [8, 16, 64])
+@pytest.mark.parametrize("H, G, D, places", [(8, 8, 64, 4), (32, 8, 64, 4), (4, 1, 64, 4), (8, 1, 64, 2), (16, 1, 64, 2), (2, 2, 128, 2), (32, 4, 128, 2), (9, 1, 128, 1),
+                                              (16, 1, 128, 1), (64, 4, 128, 1)])
+def test_single_tokens_keys_are_shared_by_as_many_ctas_as_are_resident(H, G, D, places, P):
+    """`places`: CTAs of the kernel that an SM holds, by its shared memory of up to 228 KB (a KV head of 128 with more than eight query heads: 119 KB a
+    CTA, so one) and its registers."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    for T in (1, 2, 4, 9, 18, 36, 37, 64, 100, 148, 200, 600):
+        for n in (1, 128, 500, 2048, 9000, 30000):
+            shares = shares_of_tokens(T, H, G, D, P, n)
+            assert 1 <= shares <= 16 and (shares == 1 or shares * T * G <= places * sms), (T, n, shares)
+            assert shares <= max(1, -(-n // 128))
+    assert shares_of_tokens(1, H, G, D, P, 2048) == 8
+
+
+@gpu
+@pytest.mark.parametrize("T, n", [(18, 2100), (36, 1500), (64, 900), (160, 300)])
+def test_a_kv_head_of_128_with_16_query_heads_whatever_its_shares(T, n):
+    """(Rows of one sequence at the same position: what each asks differs.)"""
+    H, G, D = 16, 1, 128
+    cache = Cache([n], G, D, 16).fill()
+    q = torch.randn(T, H, D, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16).cuda()
+    out = torch.full_like(q, 7.0)
+    pos = i32([n - 1] * T)
+    ops.attention_kv8_decode(q, cache.pool, cache.scales, out, pos, i32([0] * T), cache.table_dev, None, None, D ** -0.5, n)
+    want, sz, reach = attend(q.double(), cache.of(0), pos, None, D ** -0.5, cache.value_scales(0))
+    within(out, want, sz, reach, n, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype, P, D, places", [("f32", 16, 64, 3), ("f32", 8, 64, 3), ("f32", 12, 64, 2), ("f32", 4, 64, 2), ("f32", 16, 128, 2), ("bf16", 12, 64, 2),
+                                                  ("bf16", 4, 64, 2), ("bf16", 5, 128, 2)])
+def test_the_other_forms_keys_are_shared_by_what_its_kernels_leave_room_for(dtype, P, D, places):
+    """(The rule on the host, for 148 SMs.) Beyond what is resident only threes, where fewer than two would be and the sequences are long."""
+    code = _lib.F32 if dtype == "f32" else _lib.BF16
+    for items in (1, 3, 8, 11, 14, 20, 25, 31, 37, 42, 64, 300):
+        for n in (1, 512, 513, 1200, 2500, 30000):
+            for single in (0, 1):
+                shares = _lib.call("tk_attn_kv8_splits", items, 16, 8, D, P, code, n, n, single, 148)
+                assert shares >= 1 and (n > 512 or shares == 1) and shares <= -(-n // 256)
+                fit = places * 148 // (items * 8)
+                assert shares <= max(1, fit) or (shares == 3 and fit <= 1 and n >= 1024), (items, n, shares)
+    assert _lib.call("tk_attn_kv8_splits", 8, 16, 8, D, P, code, 4000, 4000, 1, 148) == (6 if places == 3 else 4)

@@ -486,33 +486,25 @@ TK_API int tk_attn_kv8_prefill_splits(int tokens, int items, int H, int Hkv, int
     return split;
 }
 
-// Ways to share the keys of each of `items` tiles out over CTAs, when no sequence holds more than `longest` positions and a query sees at most `reach` of them. tc:
-// single tokens through the tcgen05 kernel: as many as keep every CTA resident (four an SM for heads of 64 with up to four query heads a KV head, else two: one
-// CTA more and the launch runs in two waves), in clusters of at most eight with two tiles of 128 keys each, or of 16 with four (us by shares, 8 KV heads of 64:
-// a token behind 2,048 positions 14.9 unshared, 8.7 by 4, 7.6 by 8, 8.5 by 16; behind 30,000 136, 40, 24.7, 20.8; 8 tokens behind 32,000 49.0 by 6, 45.7 by 8, 61.7
-// by 10; 16 behind 4,000 15.3 by 4, 20.3 by 5; 64 behind up to 3,000 33.1 unshared, 38.9 by 2).
-// The mma.sync kernel's shares meet in scratch memory and cost a second launch: none up to 512 keys, then 256 keys each at least, and as many as keep every CTA
-// resident (three an SM, heads of 128 two); where two would not, but a quarter of the places is free, three of long contexts all the same (us, 32-bit,
+// Ways the mma.sync kernel shares the keys of each of `items` tiles out over CTAs, when no sequence holds more than `longest` positions and a query sees at most
+// `reach` of them; single: single tokens, whose sequences differ in length. The shares meet in scratch memory and cost a second launch: none up to 512 keys, then 256 keys
+// each at least, and as many as keep every CTA resident (three an SM for 32-bit heads of 64 whose pages come by bulk copies, else two: k8_launch's kernels have
+// 168 registers there and up to 250 elsewhere). Where two would not be resident, but a quarter of the places is free, three of long contexts all the same (us, 32-bit,
 // 8 KV heads of 64 with two query heads each: 2 prompts of up to 301 tokens 15.5 unshared, 24.0 by 2; 60 tokens behind 200 6.4 and 9.0; 256 behind 4,000 59.3, 52.1 by
-// 2, 48.7 by 3; 8 single tokens behind 4,000 34.5, 19.6 by 4, 16.8 by 6, 19.7 by 8; 64 behind 1,000 23.6, 26.8 by 2).
-TK_API int tk_attn_kv8_splits(int items, int H, int Hkv, int D, int longest, int reach, int sm_count, int tc) {
+// 2, 48.7 by 3; 8 single tokens behind 4,000 34.5, 19.6 by 4, 16.8 by 6, 19.7 by 8; 64 behind 1,000 23.6, 26.8 by 2). Keys that each lane looks up take four times as long, so
+// there it pays for single tokens from 1,024 keys, and up to an eighth more of them than the places (us, bfloat16, pages of 12: 8 behind 4,000 42.6 by 4, 52.8 by 6, which are
+// not all resident; 11 behind 1,200 24.4 by 3, 27.2 by 5; 20 behind 1,200 46.3 unshared, 43.6 by 2, 36.0 by 3; 37 behind 5,000 241 and 218 by 3; 100 tokens behind 1,000
+// 44.1 unshared, 50.5 by 2, 60.1 by 3).
+TK_API int tk_attn_kv8_splits(int items, int H, int Hkv, int D, int P, int dtype, int longest, int reach, int single, int sm_count) {
     const int64_t ctas = (int64_t)items * Hkv;
     if (ctas <= 0) return 1;
     const int64_t keys = longest < reach ? longest : reach;
-    if (!tc) {
-        const int64_t places = (int64_t)sm_count * (D == 64 ? 3 : 2);
-        int64_t n = places / ctas;
-        if (n == 1 && keys >= 2048 && 4 * ctas <= 3 * places) n = 3;
-        if (n > (keys + 255) / 256) n = (keys + 255) / 256;
-        return (int)(n < 1 || keys <= 512 ? 1 : n > 128 ? 128 : n);
-    }
-    const int64_t fit = (int64_t)sm_count * (D == 64 && H / Hkv <= 4 ? 4 : 2) / ctas, tiles = (keys + 127) / 128 + (reach < longest ? 1 : 0);
-    if (fit >= 16 && tiles >= 64) return 16;
-    int64_t n = (tiles + 1) / 2;
-    if (n < 4) n = tiles < 4 ? tiles : 4;
-    if (n > 8) n = 8;
-    if (n > fit) n = fit;
-    return (int)(n < 1 ? 1 : n);
+    const bool bulk = dtype == TK_F32 && P >= 8 && (P & (P - 1)) == 0;
+    const int64_t places = (int64_t)sm_count * (D == 64 && bulk ? 3 : 2);
+    int64_t n = places / ctas;
+    if (n <= 1 && (4 * ctas <= 3 * places ? keys >= (bulk || !single ? 2048 : 1024) : !bulk && single && keys >= 2048 && 8 * ctas <= 9 * places)) n = 3;
+    if (n > (keys + 255) / 256) n = (keys + 255) / 256;
+    return (int)(n < 1 || keys <= 512 ? 1 : n > 128 ? 128 : n);
 }
 
 // Whether single tokens of this shape take the tcgen05 kernel: 16-bit queries, pages that are a power of two and 8 or more positions.
@@ -520,6 +512,7 @@ TK_API int tk_attn_kv8_single_tc(int P, int dtype) { return dtype == TK_BF16 && 
 
 int tk_attn_kv8_tc(const void* q, const void* pool, const float* scales, void* out, const void* args, int D, cudaStream_t stream);
 int tk_attn_kv8_tc_status();
+TK_API int tk_attn_kv8_tc_splits(int items, int H, int Hkv, int D, int P, int longest, int reach);
 int tk_attn_kv8_prefill_tc(const void* q, const void* pool, const float* scales, void* out, const void* args, int D, cudaStream_t stream);
 int tk_attn_kv8_prefill_tc_status();
 
@@ -556,7 +549,7 @@ TK_API int tk_attn_kv8(const void* q, const void* pool, const float* scales, voi
         }
         const int64_t reach = window == 0 ? longest : (int64_t)(window < 0 ? -window : window) + (item_ntok != nullptr ? tokens : 0);
         const int most = (int)(reach < longest ? reach : longest);
-        nsplit = item_ntok != nullptr ? tk_attn_kv8_prefill_splits(tokens, items, H, Hkv, D, most, sms) : tk_attn_kv8_splits(items, H, Hkv, D, longest, most, sms, 1);
+        nsplit = item_ntok != nullptr ? tk_attn_kv8_prefill_splits(tokens, items, H, Hkv, D, most, sms) : tk_attn_kv8_tc_splits(items, H, Hkv, D, P, longest, most);
     }
     int shift = -1;
     if ((P & (P - 1)) == 0)

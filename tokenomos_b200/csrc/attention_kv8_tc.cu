@@ -108,6 +108,9 @@ struct K8tSmem {
     static constexpr int SCALES = BARS + (2 * STAGES + 6) * 8 + 16;                // of a tile's groups of keys: (key's, value's)
     static constexpr int MISC = SCALES + STAGES * GROUPS * 8;
     static constexpr int BYTES = MISC + (16 * 4 + 4 * 16 * 4);                     // row factors, warps' maxima or sums
+    static constexpr int BOUND = D == 64 && NR <= 4 ? 4 : 2;                       // CTAs an SM that registers are kept for
+    static constexpr int FIT = 233472 / (BYTES + 1024);                            // and that its shared memory holds (1 KB of each CTA's is the system's)
+    static constexpr int PER_SM = FIT < BOUND ? FIT : BOUND;
     static_assert(SCALES % 8 == 0 && MISC % 8 == 0, "pairs");
     // a share of the keys, for the CTAs that join theirs: [head][d] and the heads' maxima and sums, where the first tiles were
     static_assert(NR * (D + 2) * 4 <= STAGES * STAGE, "a share");
@@ -122,7 +125,7 @@ __device__ __forceinline__ uint64_t desc_keys16(uint32_t at) {
 
 // D: head size; NR: query heads a KV head has, rounded up to 2, 4, 8 or 16
 template <int D, int NR, int KG>
-__global__ void __launch_bounds__(K8T_THREADS, D == 64 && NR <= 4 ? 4 : 2)
+__global__ void __launch_bounds__(K8T_THREADS, K8tSmem<D, NR, KG>::BOUND)
 attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* out, const __grid_constant__ CUtensorMap map, const K8Args a) {
     using L = K8tSmem<D, NR, KG>;
     constexpr int GROUPS = L::GROUPS, AHEAD = 32 / GROUPS;                         // tiles whose pages and scales a copying warp's lanes know
@@ -486,40 +489,107 @@ attn_kv8_tc_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat16* o
 }
 
 template <int D, int NR, int KG>
-cudaError_t k8t_launch(const void* q, const float* scales, void* out, const CUtensorMap& map, const K8Args& a, cudaStream_t stream) {
+cudaError_t k8t_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, int64_t ctas, int nsplit, cudaStream_t stream) {
     constexpr int smem = K8tSmem<D, NR, KG>::BYTES;
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = k8_allow(attn_kv8_tc_kernel<D, NR, KG>, smem, true, done);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.items * a.Hkv * a.nsplit));
+    cfg = {};
+    cfg.gridDim = dim3((unsigned)(ctas * nsplit));
     cfg.blockDim = dim3(K8T_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
-    cfg.numAttrs = k8_attributes(attr, a.nsplit);
-    return cudaLaunchKernelEx(&cfg, attn_kv8_tc_kernel<D, NR, KG>, (const __nv_bfloat16*)q, scales, (__nv_bfloat16*)out, map, a);
+    cfg.numAttrs = k8_attributes(attr, nsplit);
+    return cudaSuccess;
 }
 
-template <int D, int KG>
-cudaError_t k8t_rows(const void* q, const float* scales, void* out, const CUtensorMap& map, const K8Args& a, cudaStream_t stream) {
-    const int G = a.H / a.Hkv;
-    return G <= 2   ? k8t_launch<D, 2, KG>(q, scales, out, map, a, stream)
-           : G <= 4 ? k8t_launch<D, 4, KG>(q, scales, out, map, a, stream)
-           : G <= 8 ? k8t_launch<D, 8, KG>(q, scales, out, map, a, stream)
-                    : k8t_launch<D, 16, KG>(q, scales, out, map, a, stream);
+struct K8tLaunch {
+    const void* q;
+    const float* scales;
+    void* out;
+    const CUtensorMap& map;
+    const K8Args& a;
+    cudaStream_t stream;
+
+    template <int D, int NR, int KG>
+    cudaError_t run() const {
+        cudaLaunchConfig_t cfg;
+        cudaLaunchAttribute attr[2];
+        const cudaError_t e = k8t_config<D, NR, KG>(cfg, attr, (int64_t)a.items * a.Hkv, a.nsplit, stream);
+        if (e != cudaSuccess) return e;
+        return cudaLaunchKernelEx(&cfg, attn_kv8_tc_kernel<D, NR, KG>, (const __nv_bfloat16*)q, scales, (__nv_bfloat16*)out, map, a);
+    }
+};
+
+// How many clusters of `n` CTAs the device holds at once, asked for once. Where an SM holds one CTA, clusters lie in whole parts of the device, 15 of 8 or 33 of 4, not 148
+// SMs' worth, and the occupancy calculator knows. (It answers one CTA an SM for every kernel that allocates tensor memory, so what several need is counted here.)
+struct K8tPlaces {
+    int n;
+    int* clusters;
+
+    template <int D, int NR, int KG>
+    cudaError_t run() const {
+        static std::atomic<int> known[16][17];
+        int device = 0, sms = 0;
+        cudaError_t e = cudaGetDevice(&device);
+        if (e != cudaSuccess) return e;
+        if (device < 16 && (*clusters = known[device][n].load(std::memory_order_relaxed)) > 0) return e;
+        if constexpr (K8tSmem<D, NR, KG>::PER_SM > 1) {
+            e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+            *clusters = K8tSmem<D, NR, KG>::PER_SM * sms / n;
+        } else {
+            cudaLaunchConfig_t cfg;
+            cudaLaunchAttribute attr[2];
+            e = k8t_config<D, NR, KG>(cfg, attr, 1, n, nullptr);
+            if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(clusters, attn_kv8_tc_kernel<D, NR, KG>, &cfg);
+        }
+        if (e == cudaSuccess && device < 16) known[device][n].store(*clusters, std::memory_order_relaxed);
+        return e;
+    }
+};
+
+template <int D, int KG, typename F>
+cudaError_t k8t_rows(int G, const F& f) {
+    return G <= 2 ? f.template run<D, 2, KG>() : G <= 4 ? f.template run<D, 4, KG>() : G <= 8 ? f.template run<D, 8, KG>() : f.template run<D, 16, KG>();
+}
+
+// f.run<D, NR, KG>() for the kernel of a layer
+template <typename F>
+cudaError_t k8t_pick(int G, int D, int P, const F& f) {
+    return P == 8 ? (D == 64 ? k8t_rows<64, 8>(G, f) : k8t_rows<128, 8>(G, f)) : (D == 64 ? k8t_rows<64, 16>(G, f) : k8t_rows<128, 16>(G, f));
 }
 
 }  // namespace
+
+// How many CTAs share each of `items` tokens' keys, when no sequence holds more than `longest` positions and a query sees at most `reach` of them: as many as keep
+// every CTA resident (one CTA more and the launch runs in two waves), in clusters of at most eight with two tiles of 128 keys each, or of 16 with four (us by
+// shares, 8 KV heads of 64: a token behind 2,048 positions 14.9 unshared, 8.7 by 4, 7.6 by 8, 8.5 by 16; behind 30,000 136, 40, 24.7, 20.8; 8 tokens behind 32,000 49.0
+// by 6, 45.7 by 8, 61.7 by 10; 16 behind 4,000 15.3 by 4, 20.3 by 5; 64 behind up to 3,000 33.1 unshared, 38.9 by 2. One KV head of 128 with 16 query heads, whose CTA fills
+// an SM: 18 tokens behind 30,000 51.2 by 6, 76.8 by 8, 82.2 by 16; 64 behind 3,000 33.0 unshared, 24.7 by 2, 33.6 by 4).
+TK_API int tk_attn_kv8_tc_splits(int items, int H, int Hkv, int D, int P, int longest, int reach) {
+    const int64_t ctas = (int64_t)items * Hkv, keys = longest < reach ? longest : reach, tiles = (keys + 127) / 128 + (reach < longest ? 1 : 0);
+    auto resident = [&](int n) {
+        int clusters = 0;
+        if (k8t_pick(H / Hkv, D, P, K8tPlaces{n, &clusters}) != cudaSuccess) {
+            cudaGetLastError();
+            return false;
+        }
+        return ctas <= clusters;
+    };
+    if (tiles >= 64 && resident(16)) return 16;
+    int n = (int)(tiles >= 16 ? 8 : (tiles + 1) / 2);
+    if (n < 4) n = tiles < 4 ? (int)tiles : 4;
+    while (n > 1 && !resident(n)) --n;
+    return n < 1 ? 1 : n;
+}
 
 // The arguments of tk_attn_kv8 for single tokens (attention_kv8.cu checks them): bfloat16, pages that are a power of two and 8 or more.
 int tk_attn_kv8_tc(const void* q, const void* pool, const float* scales, void* out, const void* args, int D, cudaStream_t stream) {
     const K8Args& a = *static_cast<const K8Args*>(args);
     CUtensorMap map = {};
     TK_CHECK_ARG(k8_map(&map, pool, D, a.P < K8T_KEYS ? a.P : K8T_KEYS), "attn_kv8: cuTensorMapEncodeTiled failed");
-    const cudaError_t e = a.P == 8 ? (D == 64 ? k8t_rows<64, 8>(q, scales, out, map, a, stream) : k8t_rows<128, 8>(q, scales, out, map, a, stream))
-                                   : (D == 64 ? k8t_rows<64, 16>(q, scales, out, map, a, stream) : k8t_rows<128, 16>(q, scales, out, map, a, stream));
+    const cudaError_t e = k8t_pick(a.H / a.Hkv, D, a.P, K8tLaunch{q, scales, out, map, a, stream});
     if (e != cudaSuccess) {
         tk_set_error("attn_kv8: launch failed: %s", cudaGetErrorString(e));
         cudaGetLastError();

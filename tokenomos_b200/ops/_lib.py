@@ -138,7 +138,7 @@ _SIGNATURES = {
     "tk_attn_kv8_prefill_supported": [I, I, I, I, I],
     "tk_attn_kv8_prefill_splits": [I, I, I, I, I, I, I],
     "tk_attn_kv8_status": [],
-    "tk_attn_kv8_splits": [I, I, I, I, I, I, I, I],
+    "tk_attn_kv8_splits": [I, I, I, I, I, I, I, I, I, I],
     "tk_attn_kv8_single_tc": [I, I],
     "tk_attn_kv8": [P, P, P, P, P, P, P, I, P, P, I, I, I, I, I, I, F, I, I, I, P, P, L, I, I, P],
     "tk_copy_rows": [P, P, P, I, P, P, I, P],

@@ -149,8 +149,8 @@ def attention_kv8_decode(q: torch.Tensor, pool: torch.Tensor, scales: torch.Tens
         T, H, Hkv, P, D, code = shape
         nsplit = 0
         if code != BF16 or not _whole_pages(P):
-            nsplit = _lib.call("tk_attn_kv8_splits", n, H, Hkv, D, int(longest), abs(int(window)) if window else int(longest),
-                               _sms(q.get_device()), 0)
+            nsplit = _lib.call("tk_attn_kv8_splits", n, H, Hkv, D, P, code, int(longest), abs(int(window)) if window else int(longest), 1,
+                               _sms(q.get_device()))
         _attend(q, pool, scales, out, positions, tok_seq, block_table, tok_index, None, n, nsplit, H // Hkv, shape, window, scale, longest,
                 gate, sink)
 
@@ -176,7 +176,7 @@ def attention_kv8_prefill(q: torch.Tensor, pool: torch.Tensor, scales: torch.Ten
         if code != BF16 or not _whole_pages(P) or not _lib.call("tk_attn_kv8_prefill_supported", H, Hkv, D, P, code):
             reach = min(int(longest), abs(int(window)) + T) if window else int(longest)
             rows = _lib.call("tk_attn_kv8_tokens", H, Hkv, D, P, code) * (H // Hkv)
-            nsplit = _lib.call("tk_attn_kv8_splits", n, H, Hkv, D, reach, reach, _sms(q.get_device()), 0)
+            nsplit = _lib.call("tk_attn_kv8_splits", n, H, Hkv, D, P, code, reach, reach, 0, _sms(q.get_device()))
         _attend(q, pool, scales, out, positions, tok_seq, block_table, tile_tok0, tile_ntok, n, nsplit, rows, shape, window, scale, longest,
                 gate, sink)
 
