@@ -184,6 +184,26 @@ def test_a_kv_head_of_128_with_16_query_heads_whatever_its_shares(T, n):
     within(out, want, sz, reach, n, torch.bfloat16)
 
 
+@gpu
+@pytest.mark.parametrize("H, G, D", [(16, 4, 128), (8, 8, 128), (32, 1, 128), (16, 4, 64), (32, 8, 64)])
+def test_portions_keys_are_shared_by_as_many_ctas_as_are_resident(H, G, D):
+    """Heads of 128 have one CTA an SM, and an eighth of the SMs or so has no room for clusters of four, nearly a fifth none for clusters of eight;
+    heads of 64 have two, and 16 of those places no room."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    for tokens in (40, 100, 128, 144, 250, 288, 544, 560, 1200, 5000):
+        tiles = -(-tokens // (128 // (H // G)))
+        for P in (8, 16):
+            for n in (300, 2500, 4200, 8300, 16000, 30000):
+                shares = _lib.lib().tk_attn_kv8_prefill_splits(tokens, tiles, H, G, D, P, n, sms)
+                ctas = shares * tiles * G
+                assert shares in (1, 2, 4, 8)
+                if D == 128:
+                    assert shares == 1 or ctas <= {2: 148, 4: 136, 8: 128}[shares], (tokens, n, shares)
+                else:
+                    assert shares == 1 or ctas <= 296 - 16 * (shares > 2) or (shares == 8 and ctas <= 296 and n >= 16384), (tokens, n, shares)
+    assert _lib.lib().tk_attn_kv8_prefill_splits(H // G, 1, H, G, D, 16, 8300, sms) == 8
+
+
 @pytest.mark.parametrize("dtype, P, D, places", [("f32", 16, 64, 3), ("f32", 8, 64, 3), ("f32", 12, 64, 2), ("f32", 4, 64, 2), ("f32", 16, 128, 2), ("bf16", 12, 64, 2),
                                                   ("bf16", 4, 64, 2), ("bf16", 5, 128, 2)])
 def test_the_other_forms_keys_are_shared_by_what_its_kernels_leave_room_for(dtype, P, D, places):

@@ -468,21 +468,28 @@ TK_API int tk_attn_kv8_prefill_supported(int H, int Hkv, int D, int P, int dtype
     return tk_attn_kv8_supported(H, Hkv, D) && dtype == TK_BF16 && P >= 8 && (P & (P - 1)) == 0;
 }
 
+int tk_attn_kv8_prefill_clusters(int D, int P, int n, int sm_count);
+
 // Tokens of one sequence a tile of tk_attn_kv8 has.
 TK_API int tk_attn_kv8_tokens(int H, int Hkv, int D, int P, int dtype) {
     return (tk_attn_kv8_prefill_supported(H, Hkv, D, P, dtype) ? 128 : K8_ROWS) / (H / Hkv);
 }
 
 // The most CTAs (1, 2, 4 or 8, a cluster) that may share one tile's keys in the tcgen05 kernel for portions, for a step of `tokens` tokens in tiles of
-// 128 / G whose list has `items` entries (a captured step's is longer than what it uses): doubled while each keeps 8 key tiles, the CTAs are
-// two an SM at most (heads of 128: one, as many as find room), and from two on, beyond one an SM, only where each keeps 32 (two CTAs of an SM walk at 0.7 of one's pace).
-TK_API int tk_attn_kv8_prefill_splits(int tokens, int items, int H, int Hkv, int D, int longest, int sm_count) {
+// 128 / G whose list has `items` entries (a captured step's is longer than what it uses): doubled while each keeps 8 key tiles, all CTAs are resident (heads of
+// 64: two an SM, 128: one), and from two on, beyond one an SM, only where each keeps 32 (two CTAs of an SM walk at 0.7 of one's pace). Eight of heads of 64 pay behind 16,384
+// positions even if the last of them wait. (us; 16 heads over 4 of 128: 128 tokens behind 8,000 39.4 by 4, 55.4 by 8, which are not resident; 288 behind 4,000 36.5 by 2, 53.8 by
+// 4. Of 64: 544 behind 7,000 44.9 by 2, 41.9 by 4; 560, of which not all are, 45.0 by 2, 60.1 by 4; 288 behind 12,000 54.9 by 4, 56.7 by 8, behind 30,000 118.7 and 106.3.)
+TK_API int tk_attn_kv8_prefill_splits(int tokens, int items, int H, int Hkv, int D, int P, int longest, int sm_count) {
     const int per_tile = 128 / (H / Hkv);
     const int64_t ctas = (int64_t)((tokens + per_tile - 1) / per_tile) * Hkv, launched = (int64_t)items * Hkv;
+    auto pays = [&](int n) {
+        return n * ctas <= (D == 64 ? 2 : 1) * (int64_t)sm_count && n * launched <= 2048 && longest >= n * 480 &&
+               (n == 2 || n * ctas <= sm_count || longest >= n * 1024) &&
+               (ctas <= tk_attn_kv8_prefill_clusters(D, P, n, sm_count) || (D == 64 && n == 8 && longest >= 16384));
+    };
     int split = 1;
-    while (split < 8 && 2 * split * ctas <= (D == 64 ? 2 : 1) * (int64_t)sm_count && 2 * split * launched <= 2048 && longest >= 2 * split * 480 &&
-           (split == 1 || 2 * split * ctas <= sm_count || longest >= split * 2048))
-        split *= 2;
+    while (split < 8 && pays(2 * split)) split *= 2;
     return split;
 }
 
@@ -549,7 +556,7 @@ TK_API int tk_attn_kv8(const void* q, const void* pool, const float* scales, voi
         }
         const int64_t reach = window == 0 ? longest : (int64_t)(window < 0 ? -window : window) + (item_ntok != nullptr ? tokens : 0);
         const int most = (int)(reach < longest ? reach : longest);
-        nsplit = item_ntok != nullptr ? tk_attn_kv8_prefill_splits(tokens, items, H, Hkv, D, most, sms) : tk_attn_kv8_tc_splits(items, H, Hkv, D, P, longest, most);
+        nsplit = item_ntok != nullptr ? tk_attn_kv8_prefill_splits(tokens, items, H, Hkv, D, P, most, sms) : tk_attn_kv8_tc_splits(items, H, Hkv, D, P, longest, most);
     }
     int shift = -1;
     if ((P & (P - 1)) == 0)

@@ -533,22 +533,58 @@ attn_kv8_prefill_kernel(const __nv_bfloat16* q, const float* scales, __nv_bfloat
 }
 
 template <int D, int KG>
-cudaError_t kp_launch(const void* q, const float* scales, void* out, const CUtensorMap& map, const K8Args& a, cudaStream_t stream) {
+cudaError_t kp_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, int64_t ctas, int nsplit, cudaStream_t stream) {
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = k8_allow(attn_kv8_prefill_kernel<D, KG>, KpSmem<D, KG>::BYTES, false, done);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.items * a.Hkv * a.nsplit));
+    cfg = {};
+    cfg.gridDim = dim3((unsigned)(ctas * nsplit));
     cfg.blockDim = dim3(KP_THREADS);
     cfg.dynamicSmemBytes = KpSmem<D, KG>::BYTES;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
-    cfg.numAttrs = k8_attributes(attr, a.nsplit);
+    cfg.numAttrs = k8_attributes(attr, nsplit);
+    return cudaSuccess;
+}
+
+template <int D, int KG>
+cudaError_t kp_launch(const void* q, const float* scales, void* out, const CUtensorMap& map, const K8Args& a, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[2];
+    const cudaError_t e = kp_config<D, KG>(cfg, attr, (int64_t)a.items * a.Hkv, a.nsplit, stream);
+    if (e != cudaSuccess) return e;
     return cudaLaunchKernelEx(&cfg, attn_kv8_prefill_kernel<D, KG>, (const __nv_bfloat16*)q, scales, (__nv_bfloat16*)out, map, a);
 }
 
+// clusters of n CTAs that a device with one CTA an SM holds, asked for once (n: 2, 4 or 8)
+template <int D, int KG>
+cudaError_t kp_clusters(int n, int* clusters) {
+    static std::atomic<int> known[16][9];
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess || (device < 16 && (*clusters = known[device][n].load(std::memory_order_relaxed)) > 0)) return e;
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[2];
+    e = kp_config<D, KG>(cfg, attr, 1, n, nullptr);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(clusters, attn_kv8_prefill_kernel<D, KG>, &cfg);
+    if (e == cudaSuccess && device < 16) known[device][n].store(*clusters, std::memory_order_relaxed);
+    return e;
+}
+
 }  // namespace
+
+// How many clusters of n CTAs (2, 4 or 8) are resident at once. Heads of 128 fill an SM's tensor memory with one CTA, and clusters lie in whole parts of the device: the
+// occupancy calculator says 74 of 2, 33 of 4, 15 of 8 for 148 SMs. It says the same of heads of 64, which have two CTAs an SM (it takes a kernel that allocates tensor
+// memory for one a SM): there pairs fill the device, and clusters of 4 and 8 all but 16 of its places by measurement (68 of 4 run together, 72 do not).
+int tk_attn_kv8_prefill_clusters(int D, int P, int n, int sm_count) {
+    if (D == 64) return (2 * sm_count - (n > 2 ? 16 : 0)) / n;
+    int clusters = 0;
+    if ((P == 8 ? kp_clusters<128, 8>(n, &clusters) : kp_clusters<128, 16>(n, &clusters)) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    return clusters;
+}
 
 // The arguments of tk_attn_kv8 for tiles (attention_kv8.cu checks them): bfloat16, pages that are a power of two and 8 or more.
 int tk_attn_kv8_prefill_tc(const void* q, const void* pool, const float* scales, void* out, const void* args, int D, cudaStream_t stream) {

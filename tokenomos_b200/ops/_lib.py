@@ -136,7 +136,6 @@ _SIGNATURES = {
     "tk_attn_kv8_supported": [I, I, I],
     "tk_attn_kv8_tokens": [I, I, I, I, I],
     "tk_attn_kv8_prefill_supported": [I, I, I, I, I],
-    "tk_attn_kv8_prefill_splits": [I, I, I, I, I, I, I],
     "tk_attn_kv8_status": [],
     "tk_attn_kv8_splits": [I, I, I, I, I, I, I, I, I, I],
     "tk_attn_kv8_single_tc": [I, I],
@@ -197,7 +196,7 @@ _QUERIES = {"tk_check_device", "tk_built_for", "tk_set_pdl", "tk_checks_enabled"
             "tk_attn_pointwise_mma_tokens", "tk_ssd_max_state", "tk_ssd_split", "tk_linmem_max_dim", "tk_linmem_scratch", "tk_delta_chunks_scratch",
             "tk_attn_biased_mma_supported", "tk_attn_biased_mma_tokens", "tk_gemm_stream32_max_rows",
             "tk_gemm_split32_status", "tk_attn_f32_supported", "tk_attn_f32_tokens", "tk_ssd_chunked_scratch", "tk_ssd_tc_scratch",
-            "tk_attn_kv8_supported", "tk_attn_kv8_tokens", "tk_attn_kv8_splits", "tk_attn_kv8_single_tc", "tk_attn_kv8_prefill_supported", "tk_attn_kv8_prefill_splits",
+            "tk_attn_kv8_supported", "tk_attn_kv8_tokens", "tk_attn_kv8_splits", "tk_attn_kv8_single_tc", "tk_attn_kv8_prefill_supported",
             "tk_attn_kv8_status"}
 
 
