@@ -326,15 +326,15 @@ qk_norm_rope_write8_kernel(const T* qkv, int64_t qkv_stride, T* q_out, uint8_t* 
 }  // namespace
 
 // qkv: [T, (H + 2 Hkv) D] with row stride `qkv_stride`, 16-byte aligned rows; pool: [pages, 2, Hkv, P, D] bytes, scales: [pages, 2, Hkv]. wq / wk:
-// both or neither, D floats at any float's address. freq: [R / 2]. The tokens of a sequence lie side by side in the step, at consecutive positions.
+// both or neither, D floats at any float's address. Hkv 0: queries only (no pool, scales, tables nor wk). freq: [R / 2]. The tokens of a sequence lie side by side in the step, at consecutive positions.
 TK_API int tk_qk_norm_rope_write8(const void* qkv, int64_t qkv_stride, void* q_out, void* pool, float* scales, const float* wq,
                                   const float* wk, float eps, const float* freq, float cs_mult, int interleaved, const int* positions,
                                   const int* tok_seq, const int* block_table, int bt_stride, int T_, int H, int Hkv, int D, int R, int P,
                                   int dtype, cudaStream_t stream) {
-    TK_CHECK_ARG(T_ >= 0 && H > 0 && Hkv > 0 && P > 0 && bt_stride >= 0, "qk_norm_rope_write8: bad sizes");
+    TK_CHECK_ARG(T_ >= 0 && H > 0 && Hkv >= 0 && P > 0 && bt_stride >= 0, "qk_norm_rope_write8: bad sizes");
     TK_CHECK_ARG(D == 64 || D == 128, "qk_norm_rope_write8: heads of %d (64 and 128 are built)", D);
     TK_CHECK_ARG(R >= 0 && R <= D && R % 2 == 0, "qk_norm_rope_write8: rotary width %d of head %d", R, D);
-    TK_CHECK_ARG((wq == nullptr) == (wk == nullptr), "qk_norm_rope_write8: q and k norms come together");
+    TK_CHECK_ARG(Hkv == 0 || (wq == nullptr) == (wk == nullptr), "qk_norm_rope_write8: q and k norms come together");
     TK_CHECK_ARG(dtype == TK_F32 || dtype == TK_BF16, "qk_norm_rope_write8: unknown dtype %d", dtype);
     const int vec = dtype == TK_F32 ? 4 : 8;
     TK_CHECK_ARG(qkv_stride % vec == 0 && (uintptr_t)qkv % 16 == 0 && (uintptr_t)q_out % 16 == 0 && (uintptr_t)pool % 16 == 0,

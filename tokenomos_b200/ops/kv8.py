@@ -60,34 +60,42 @@ def kv8_supported(heads: int, kv_heads: int, head_dim: int) -> bool:
     return bool(_lib.call("tk_attn_kv8_supported", heads, kv_heads, head_dim))
 
 
-def qk_norm_rope_write8(qkv: torch.Tensor, pool: torch.Tensor, scales: torch.Tensor, wq: torch.Tensor | None,
+def qk_norm_rope_write8(qkv: torch.Tensor, pool: torch.Tensor | None, scales: torch.Tensor | None, wq: torch.Tensor | None,
                         wk: torch.Tensor | None, eps: float, inv_freq: torch.Tensor, positions: torch.Tensor,
-                        tok_seq: torch.Tensor, block_table: torch.Tensor, heads: int, kv_heads: int, head_dim: int, page: int,
+                        tok_seq: torch.Tensor, block_table: torch.Tensor | None, heads: int, kv_heads: int, head_dim: int, page: int,
                         cs_mult: float = 1.0, interleaved: bool = False) -> torch.Tensor:
     """``qk_norm_rope_write`` for an 8-bit cache: norm (``wq``, ``wk``: both or neither) and rotate the q and k heads of
     ``qkv`` [T, (H + 2 Hkv) D] (rows may be strided); returns q [T, H, D] and writes k and v into ``pool`` and ``scales`` at each token's
     position. ``inv_freq`` [R / 2]: the first R columns are rotated, pairs (i, i + R / 2), or (2i, 2i + 1) when
-    ``interleaved``; cos and sin are multiplied by ``cs_mult``. Everything is 32-bit (angles 64-bit) and rounded once.
+    ``interleaved``; cos and sin are multiplied by ``cs_mult``. Everything is 32-bit (an angle in two 32-bit numbers) and rounded once; a head whose
+    squares overflow 32 bits is 0, as in ``qk_norm_rope_write``. ``kv_heads`` 0: queries only (the layer reads another layer's cache).
 
     A sequence's tokens lie side by side in the step, at consecutive positions (negative ones are not written), and a page that tokens are written into
     belongs to one sequence. A block that already holds tokens of earlier steps keeps its scale or raises it, and then its earlier bytes are
     rounded to the new one (which changes nothing above 2^-6 of it, e4m3's smallest normal number)."""
     name = "qk_norm_rope_write8"
     _here(name, qkv, pool, scales, wq, wk, inv_freq, positions, tok_seq, block_table)
-    if _check_cache(name, pool, scales) != (kv_heads, page, head_dim):
-        raise KernelError(f"{name}: cache {tuple(pool.shape)} does not match [pages, 2, {kv_heads}, {page}, {head_dim}]")
     if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] != (heads + 2 * kv_heads) * head_dim:
         raise KernelError(f"{name}: qkv {tuple(qkv.shape)} for {heads}+2*{kv_heads} heads of {head_dim}")
     code = ops._dtype_code(qkv)
     T = qkv.shape[0]
-    _check_layout(name, T, positions, tok_seq, block_table)
+    if kv_heads:
+        if pool is None or scales is None or block_table is None:
+            raise KernelError(f"{name}: keys need a cache, its scales and a block table")
+        if _check_cache(name, pool, scales) != (kv_heads, page, head_dim):
+            raise KernelError(f"{name}: cache {tuple(pool.shape)} does not match [pages, 2, {kv_heads}, {page}, {head_dim}]")
+        _check_layout(name, T, positions, tok_seq, block_table)
+    else:
+        pool = scales = block_table = wk = None
+        if ops._i32(positions, "positions").numel() < T:
+            raise KernelError(f"{name}: positions is shorter than the {T} rows")
     rot = 2 * inv_freq.numel()
     ops._f32vec(inv_freq, "inv_freq", rot // 2)
     q = qkv.new_empty((T, heads, head_dim))
-    _lib.call("tk_qk_norm_rope_write8", qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1], q.data_ptr(), pool.data_ptr(),
-              scales.data_ptr(), ops._ptr(ops._f32vec(wq, "q_norm weight", head_dim)), ops._ptr(ops._f32vec(wk, "k_norm weight", head_dim)),
+    _lib.call("tk_qk_norm_rope_write8", qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1], q.data_ptr(), ops._ptr(pool),
+              ops._ptr(scales), ops._ptr(ops._f32vec(wq, "q_norm weight", head_dim)), ops._ptr(ops._f32vec(wk, "k_norm weight", head_dim)),
               float(eps), inv_freq.data_ptr(), float(cs_mult), int(bool(interleaved)), positions.data_ptr(), tok_seq.data_ptr(),
-              block_table.data_ptr(), block_table.stride(0), T, heads, kv_heads, head_dim, rot, page, code, ops._stream())
+              ops._ptr(block_table), block_table.stride(0) if kv_heads else 0, T, heads, kv_heads, head_dim, rot, page, code, ops._stream())
     return q
 
 

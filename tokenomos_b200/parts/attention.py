@@ -400,10 +400,7 @@ class Attention:
 
     def _core8(self, qkv, pool, scales, table, ctx: StepContext, gate) -> torch.Tensor:
         """``_core`` over an 8-bit cache: prompt portions in tiles, single tokens with their keys shared out over CTAs."""
-        if self.head_layout.kv_heads:
-            q = self.rope.encode_qk8(qkv, ctx, self.head_layout, pool, scales, table)
-        else:
-            q = self.rope.encode_qk(qkv, ctx, self.head_layout, None, None)
+        q = self.rope.encode_qk8(qkv, ctx, self.head_layout, pool, scales, table)
         out = torch.empty_like(q)
         by_head = gate if self.gate_kind == "head" else None
         if not ctx.host.decode_only:

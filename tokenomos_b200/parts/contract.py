@@ -344,5 +344,12 @@ class PositionEncoding(Protocol):
     # ``encode_qk``; both ways give the same bits. Encodings without the method are always
     # called through ``encode_qk``.
     #
+    # Optional. An encoding that writes an 8-bit cache has
+    #
+    #     def encode_qk8(self, qkv, ctx, heads, pool, scales, table) -> torch.Tensor
+    #
+    # which does what ``encode_qk`` does into ``pool`` (e4m3) and ``scales`` [pages, 2, Hkv]; with ``heads.kv_heads`` 0 it returns
+    # the queries alone, as the layer whose cache is read forms its own.
+    #
     # Optional. An encoding that writes values mixed with another layer's (``encode_qk(..., mix=ValueRows)``)
     # says so with ``takes_value_mix = True``.

@@ -49,7 +49,8 @@ class Rope:
 
     def encode_qk8(self, qkv: torch.Tensor, ctx: StepContext, heads: HeadLayout, pool: torch.Tensor, scales: torch.Tensor,
                    table: torch.Tensor) -> torch.Tensor:
-        """``encode_qk`` for an 8-bit cache (cos and sin, and everything before the quantisation, stay 32-bit)."""
+        """``encode_qk`` for an 8-bit cache (cos and sin, and everything before the quantisation, stay 32-bit); of a layer without keys of its own
+        the queries alone."""
         return ops.qk_norm_rope_write8(qkv, pool, scales, heads.q_norm, heads.k_norm, heads.eps, self.inv_freq, ctx.positions,
                                        ctx.tok_seq, table, heads.heads, heads.kv_heads, heads.head_dim, ctx.page_size)
 
