@@ -86,3 +86,15 @@ def test_keys_without_a_cache_are_refused():
         ops.qk_norm_rope_write8(x, None, None, None, None, 0.0, f, one, one, None, 2, 1, 64, 16)
     with pytest.raises(KernelError, match="shorter"):
         ops.qk_norm_rope_write8(x, None, None, None, None, 0.0, f, one[:0], one, None, 4, 0, 64, 16)
+
+
+# ---- what is refused when a layer is built ----
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, float("nan")])
+def test_a_factor_of_the_scores_that_is_not_positive_is_refused(scale):
+    from tokenomos_b200.parts.rope import Rope
+
+    rope = Rope(64, 32, 1e4, "cpu")
+    assert attention(4, 2, 64, 16, rope, device="cpu", scale=0.5).scale == 0.5
+    with pytest.raises(ValueError, match="positive"):
+        attention(4, 2, 64, 16, rope, device="cpu", scale=scale)

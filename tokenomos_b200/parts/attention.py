@@ -166,6 +166,8 @@ class Attention:
                                  "a KV head)")
             if not hasattr(rope, "encode_qk8") or (kv_source is None and (q_norm is None) != (k_norm is None)):
                 raise ValueError("attention: an 8-bit cache needs a position part that writes it, and q and k norms both or neither")
+            if scale is not None and not scale > 0:
+                raise ValueError(f"attention: over an 8-bit cache the scores' factor is positive, not {scale}")
         # what the one-kernel decode form and the norms folded into the projections do not take
         # (the tensor-core kernels take all of it but a value size of its own; the general
         # kernel takes everything)
