@@ -98,3 +98,18 @@ def test_a_factor_of_the_scores_that_is_not_positive_is_refused(scale):
     assert attention(4, 2, 64, 16, rope, device="cpu", scale=0.5).scale == 0.5
     with pytest.raises(ValueError, match="positive"):
         attention(4, 2, 64, 16, rope, device="cpu", scale=scale)
+
+
+@pytest.mark.parametrize("which", ["q", "k", "both"])
+def test_rotary_refuses_norms_over_either_cache(which):
+    """(Nothing is launched: the check comes first.)"""
+    from tokenomos_b200.parts.contract import HeadLayout
+    from tokenomos_b200.parts.rope import Rotary
+
+    w = torch.ones(64)
+    heads = HeadLayout(4, 2, 64, w if which != "k" else None, w if which != "q" else None, 1e-5)
+    rotary = Rotary(64, 64, 1e4, "half", None, "cpu")
+    with pytest.raises(ValueError, match="norms"):
+        rotary.encode_qk(torch.zeros(1, 8 * 64), None, heads, None, None)
+    with pytest.raises(ValueError, match="norms"):
+        rotary.encode_qk8(torch.zeros(1, 8 * 64), None, heads, None, None, None)

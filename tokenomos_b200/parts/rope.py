@@ -118,10 +118,14 @@ class Rotary:
         of its own (attention does, in steps where every sequence brings one token)."""
         return self.freq, self.cs_mult, self.interleaved
 
-    def encode_qk(self, qkv: torch.Tensor, ctx: StepContext, heads: HeadLayout,
-                  pool: torch.Tensor | None, table: torch.Tensor | None) -> torch.Tensor:
+    @staticmethod
+    def _check_norms(heads: HeadLayout) -> None:
         if heads.q_norm is not None or heads.k_norm is not None:
             raise ValueError("Rotary: per-head q/k norms are the 'rope' encoding's")
+
+    def encode_qk(self, qkv: torch.Tensor, ctx: StepContext, heads: HeadLayout,
+                  pool: torch.Tensor | None, table: torch.Tensor | None) -> torch.Tensor:
+        self._check_norms(heads)
         return ops.rotary_write(qkv, pool, self.freq, self.cs_mult, ctx.positions, ctx.tok_seq, table,
                                 heads.heads, heads.kv_heads, heads.head_dim,
                                 heads.v_dim if heads.v_dim is not None else heads.head_dim, ctx.page_size,
@@ -131,6 +135,7 @@ class Rotary:
     def encode_qk8(self, qkv: torch.Tensor, ctx: StepContext, heads: HeadLayout, pool: torch.Tensor, scales: torch.Tensor,
                    table: torch.Tensor) -> torch.Tensor:
         """``encode_qk`` for an 8-bit cache."""
+        self._check_norms(heads)
         return ops.qk_norm_rope_write8(qkv, pool, scales, heads.q_norm, heads.k_norm, heads.eps, self.freq, ctx.positions,
                                        ctx.tok_seq, table, heads.heads, heads.kv_heads, heads.head_dim, ctx.page_size,
                                        self.cs_mult, self.interleaved)
