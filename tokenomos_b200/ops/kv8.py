@@ -9,6 +9,7 @@ head). A byte stands for ``scale * e4m3``; a block's scale is the smallest with 
 from __future__ import annotations
 
 import array
+import functools
 from typing import Sequence
 
 import torch
@@ -137,9 +138,16 @@ def _attend(q, pool, scales, out, positions, tok_seq, block_table, tok0, ntok, i
               1 if sink else 0, code, ops._stream())
 
 
-def _whole_pages(P: int) -> bool:
-    """Whether pages are a power of two and 8 positions or more, as the tcgen05 kernels take them."""
-    return P >= 8 and not P & (P - 1)
+@functools.lru_cache(maxsize=None)
+def _decode_chooses(page: int, code: int) -> bool:
+    """Whether the entry point chooses the shares of single tokens itself (the tcgen05 kernel, which needs no scratch memory)."""
+    return bool(_lib.call("tk_attn_kv8_single_tc", page, code))
+
+
+@functools.lru_cache(maxsize=None)
+def _prefill_chooses(heads: int, kv_heads: int, head_dim: int, page: int, code: int) -> bool:
+    """The same of prompt portions."""
+    return bool(_lib.call("tk_attn_kv8_prefill_supported", heads, kv_heads, head_dim, page, code))
 
 
 def attention_kv8_decode(q: torch.Tensor, pool: torch.Tensor, scales: torch.Tensor, out: torch.Tensor, positions: torch.Tensor,
@@ -156,7 +164,7 @@ def attention_kv8_decode(q: torch.Tensor, pool: torch.Tensor, scales: torch.Tens
     if n:
         T, H, Hkv, P, D, code = shape
         nsplit = 0
-        if code != BF16 or not _whole_pages(P):
+        if not _decode_chooses(P, code):
             nsplit = _lib.call("tk_attn_kv8_splits", n, H, Hkv, D, P, code, int(longest), abs(int(window)) if window else int(longest), 1,
                                _sms(q.get_device()))
         _attend(q, pool, scales, out, positions, tok_seq, block_table, tok_index, None, n, nsplit, H // Hkv, shape, window, scale, longest,
@@ -181,7 +189,7 @@ def attention_kv8_prefill(q: torch.Tensor, pool: torch.Tensor, scales: torch.Ten
         raise KernelError(f"{name}: {n} first tokens for {tile_ntok.numel()} tiles")
     if n:
         nsplit = rows = 0
-        if code != BF16 or not _whole_pages(P) or not _lib.call("tk_attn_kv8_prefill_supported", H, Hkv, D, P, code):
+        if not _prefill_chooses(H, Hkv, D, P, code):
             reach = min(int(longest), abs(int(window)) + T) if window else int(longest)
             rows = _lib.call("tk_attn_kv8_tokens", H, Hkv, D, P, code) * (H // Hkv)
             nsplit = _lib.call("tk_attn_kv8_splits", n, H, Hkv, D, P, code, reach, reach, 0, _sms(q.get_device()))
