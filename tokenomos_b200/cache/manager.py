@@ -364,7 +364,7 @@ class CacheManager:
         if taken or len(set(children)) != len(children):
             raise CacheError(f"requests {taken or children!r} are already live")
         full, part = divmod(st.length, self.page_size)
-        if len(self.slots) < len(children) or (part and self.free_pages() < len(children)):
+        if len(self.slots) < len(children) or self.free_pages() < self.fork_pages(rid) * len(children):
             raise OutOfPages(f"{len(children)} forks of request {rid!r} need a slot each" + (" and a page of each group" if part else ""))
         copies: list[RequestState] = []
         for child in children:
