@@ -89,14 +89,14 @@ __device__ __forceinline__ bool any_of_128(bool mine) {
 }
 __device__ __forceinline__ void sync_128() { asm volatile("bar.sync 2, 128;" ::: "memory"); }
 
-// tiles of keys and values in shared memory (they leave room for three CTAs an SM, heads of 128 for two)
-template <int D>
-constexpr int k8t_stages = 3;
+// tiles of keys and values in shared memory (they leave room for four CTAs an SM where a KV head of 64 has up to four query heads, else for two, and for one of
+// heads of 128 with more than eight)
+constexpr int K8T_STAGES = 3;
 
 template <int D, int NR, int KG>
 struct K8tSmem {
     static constexpr int GROUPS = K8T_KEYS / KG;                                   // that share scales: 16 keys, or 8 where a page has no more
-    static constexpr int STAGES = k8t_stages<D>;
+    static constexpr int STAGES = K8T_STAGES;
     static constexpr int S_COLS = 2 * NR < 16 ? 16 : 2 * NR;                       // scores' columns: term, head
     static constexpr int O_COLS = 4 * NR < 16 ? 16 : 4 * NR;                       // outputs' columns: term, head
     static constexpr int P_BYTES = O_COLS * K8T_KEYS;                              // [term, head / 16][key][16]
