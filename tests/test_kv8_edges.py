@@ -120,6 +120,30 @@ def test_a_prompts_last_row_and_the_same_token_decoded_agree(share, dtype):
             assert (out[:, r] - want).norm() <= 1.25 * mean.sqrt()
 
 
+# ---- queries that are not finite ----
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("P", [16, 8, 12])
+@pytest.mark.parametrize("new", [1, 20])
+@pytest.mark.parametrize("what", [math.inf, -math.inf, math.nan])
+def test_a_row_whose_query_is_not_finite_is_nan_and_no_other(what, new, P, dtype):
+    """Keys whose first element is negative (none is 0): an infinite query element makes minus infinity of every score, and a softmax of those is no
+    number."""
+    H, G, D, n = 4, 2, 64, 90
+    cache = Cache([n], G, D, P).fill()
+    pages = cache.table[0].long().cuda()
+    cache.pool.view(torch.uint8)[pages, 0, :, :, 0] = torch.tensor(-64.0).to(torch.float8_e4m3fn).view(torch.uint8).item()
+    q = torch.randn(new, H, D, generator=torch.Generator().manual_seed(0)).to(dtype).cuda()
+    clean, _ = run_attention(cache, q, [new], None, 0.125)
+    bad = q.clone()
+    bad[-1, 2, 0] = what
+    out, _ = run_attention(cache, bad, [new], None, 0.125)
+    assert out[-1, 2].isnan().all()
+    out[-1, 2] = clean[-1, 2]
+    assert torch.equal(out, clean) and torch.isfinite(clean).all()
+
+
 # ---- norms ----
 
 @gpu

@@ -107,10 +107,12 @@ attn_kv8_kernel(const T* q, const uint8_t* pool, const float* scales, T* out, co
         }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        // a row's largest element to [2^14, 2^15) (a row that is not finite stays as it is)
+        // a row's largest element to [2^14, 2^15); of a row with an infinite element every score is NaN (minus infinities alone would pass for a row that
+        // sees nothing), as one NaN makes it by itself
         int e2 = (__float_as_int(most) >> 23) - 127;
-        e2 = e2 > 127 || most == 0.f ? 14 : max(e2, -100);
-        const float up = exp2i(14 - e2);
+        const bool fine = e2 <= 127;
+        e2 = !fine || most == 0.f ? 14 : max(e2, -100);
+        const float up = fine ? exp2i(14 - e2) : NAN;
         row_c[hrow] = a.scale * K8_LOG2E * exp2i(e2 - 14);
         row_pos[hrow] = valid ? pos_first + r / G : -1;
 #pragma unroll
