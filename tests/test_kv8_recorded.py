@@ -20,8 +20,8 @@ FORMS = [(BF16, 16, False), (BF16, 8, False), (F32, 16, True), (F32, 8, True), (
 class Call:
     """One call of either form over a cache of its own: sequences of up to `longest` positions, their last `new` tokens."""
 
-    def __init__(self, dtype, P, new, D, seed, lens=(2600, 1900)):
-        self.H, self.G, self.D, self.P, self.new, self.lens = 4, 1, D, P, new, list(lens)
+    def __init__(self, dtype, P, new, D, seed, lens=(2600, 1900), H=4):
+        self.H, self.G, self.D, self.P, self.new, self.lens = H, 1, D, P, new, list(lens)
         self.cache = Cache(self.lens, self.G, D, P, seed=seed).fill(seed)
         gen = torch.Generator().manual_seed(seed)
         T = new * len(self.lens)
@@ -138,3 +138,32 @@ def test_a_recorded_write_follows_its_inputs(dtype, T):
         want = run(b)
         assert torch.equal(q, want) and torch.equal(a.pool.view(torch.uint8), b.pool.view(torch.uint8))
         assert torch.equal(a.scales.view(torch.int32), b.scales.view(torch.int32))
+
+
+FIRST = """
+import sys
+sys.path.insert(0, "tests")
+import torch
+from test_kv8_recorded import Call
+call = Call(torch.bfloat16, 16, int(sys.argv[1]), 128, 0, H=16)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    call()
+g.replay()
+torch.cuda.synchronize()
+call.check()
+print("fine")
+"""
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 30])
+def test_a_process_may_record_its_first_call(new):
+    """What the entry points ask of the device once (attributes, places) may be asked while a stream is being recorded."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    done = subprocess.run([sys.executable, "-c", FIRST, str(new)], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and done.stdout.strip() == "fine", done.stdout + done.stderr
