@@ -25,8 +25,9 @@
 // Masked keys and values are never read (their bytes are zero in the products), so what an unwritten part of a page holds does not
 // matter. A row that sees no key is 0.
 //
-// Measured (32-bit, 16 heads over 8 of 64, one B200): two prompts of up to 301 tokens 15.5 us, 1,000 tokens 31.3, 8 single tokens behind 4,000 positions 16.9 (2.0 TB/s), one
-// behind 2,000 9.3. Bound by latency: 160 registers leave three CTAs an SM (the two prompts in two shares each 23.9 us, with two CTAs 27.3; units of 16 keys allow four: 12.9 for the two prompts, but 34.6 for the
+// Measured (32-bit, 16 heads over 8 of 64, one B200): two prompts of up to 301 tokens 15.6 us, 1,000 tokens 31.4, 8 single tokens behind up to 4,000 positions 17.0 (1.7 TB/s), one
+// behind 2,000 9.4. Keys that each lane looks up (bfloat16, 32 heads over 8 of 64, pages of 12): 1,000 tokens 166, 256 behind 4,000 304, 8 single tokens behind up to 4,000 42.7; 64 behind up to 1,000, pages
+// of 4, 70.5. Bound by latency: 168 registers leave three CTAs an SM (the two prompts in two shares each 23.9 us, with two CTAs 27.3; units of 16 keys allow four: 12.9 for the two prompts, but 34.6 for the
 // 1,000 tokens and 49.5 for 34.5 unshared single tokens). A warp a row tile instead of a share of a CTA's keys was slower for prompts.
 #include <math.h>
 

@@ -23,8 +23,9 @@
 //   warps 0-3   thread = key: masks, reference maximum (one vote of the four warps a tile), weights, their terms into shared memory
 //               ([term and head][key], the second product's other operand); positions that are not to be seen have their value rows zeroed there
 //
-// Measured (one B200, pages of 16): one token behind 2,048 positions 7.7 us and 64 behind up to 3,000 32.5 (32 heads over 8 of 64; 9.9 and 69 on mma.sync), 8
-// behind 32,000 45.5 (16 heads over 8: 5.7 TB/s; 109), 16 behind a window of 1,024 9.3 (16 heads over 4 of 128; 16.3). HBM bounds long contexts (7 TB/s while all of
+// Measured (one B200, pages of 16): one token behind 2,048 positions 7.7 us and 64 behind up to 3,000 32.3 (32 heads over 8 of 64; 9.9 and 69 on mma.sync), 8
+// behind 32,000 45.2 (16 heads over 8: 5.7 TB/s; 109), 16 behind a window of 1,024 9.2 (16 heads over 4 of 128; 16.3), 64 behind up to 3,000 of one KV head of 128 with
+// 16 query heads 24.7 (floor 5.8: one CTA an SM, 128 registers a thread and what they spill). HBM bounds long contexts (7 TB/s while all of
 // the 64's CTAs work, 2,240 cycles a tile; then the longest ones end alone); below
 // some 8 MB of cache the launch, the chain of a tile's products and weights and the shares' joining are what there is. Tried and slower or no faster: two or four to six tiles
 // ahead, four copying warps or one (65-100 cycles a load, one after the other within a warp), the shares joined through global memory,

@@ -16,7 +16,7 @@
 // of their own take the heads of one token, or of four where there are many. Large steps take CTAs of 8 warps (two KV heads each).
 //
 // Measured (one B200, 32 heads over 8 of 64): 8 single tokens 3.0 us, a prompt of 2,048 tokens 11.4 (3.5 us of them its bytes' at HBM's rate), three portions of 333 tokens of the
-// 32-bit model (16 heads over 8) 5.4. Bound by its chain of dependent loads (tokens, page, rows) at decode sizes, by instructions in long prompts (2.3 of 4 a cycle).
+// 32-bit model (16 heads over 8) 5.5. Bound by its chain of dependent loads (tokens, page, rows) at decode sizes, by instructions in long prompts (2.3 of 4 a cycle).
 #include <math.h>
 
 #include <algorithm>
