@@ -194,6 +194,25 @@ def test_single_tokens_keys_are_shared_by_as_many_ctas_as_are_resident(H, G, D, 
     assert shares_of_tokens(1, H, G, D, P, 2048) == 8
 
 
+# the most clusters of 3, 4, ... CTAs that ran together on a B200's 148 SMs, by CTAs an SM (one more, and a launch took half as long again)
+TOGETHER = {1: {2: 74, 3: 45, 4: 33, 5: 26, 6: 22, 7: 15, 8: 15, 16: 7}, 2: {2: 148, 3: 92, 4: 70, 5: 56, 6: 45, 7: 37, 8: 33, 16: 14},
+            4: {2: 296, 3: 185, 4: 140, 5: 112, 6: 92, 7: 76, 8: 66, 16: 28}}
+
+
+@gpu
+@pytest.mark.parametrize("H, G, D, places", [(4, 1, 64, 4), (4, 2, 64, 4), (8, 1, 64, 2), (16, 1, 64, 2), (8, 2, 128, 2), (16, 1, 128, 1)])
+def test_clusters_of_single_tokens_leave_the_places_empty_that_they_cannot_fill(H, G, D, places):
+    if torch.cuda.get_device_properties(0).multi_processor_count != 148:
+        pytest.skip("counted on 148 SMs")
+    for T in range(1, 310 // G):
+        for n in (500, 900, 2000, 4000, 9000, 30000):
+            shares = shares_of_tokens(T, H, G, D, 16, n)
+            assert shares == 1 or T * G <= TOGETHER[places][shares], (T, n, shares)
+    # and those that they can
+    for want, n in ((4, 500), (8, 4000), (16, 9000)):
+        assert shares_of_tokens(TOGETHER[places][want] * 9 // 10 // G, H, G, D, 16, n) == want
+
+
 @gpu
 @pytest.mark.parametrize("T, n", [(18, 2100), (36, 1500), (64, 900), (160, 300)])
 def test_a_kv_head_of_128_with_16_query_heads_whatever_its_shares(T, n):

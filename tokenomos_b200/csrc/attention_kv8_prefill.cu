@@ -574,10 +574,9 @@ cudaError_t kp_clusters(int n, int* clusters) {
 }  // namespace
 
 // How many clusters of n CTAs (2, 4 or 8) are resident at once. Heads of 128 fill an SM's tensor memory with one CTA, and clusters lie in whole parts of the device: the
-// occupancy calculator says 74 of 2, 33 of 4, 15 of 8 for 148 SMs. It says the same of heads of 64, which have two CTAs an SM (it takes a kernel that allocates tensor
-// memory for one a SM): there pairs fill the device, and clusters of 4 and 8 all but 16 of its places by measurement (68 of 4 run together, 72 do not).
+// occupancy calculator says 74 of 2, 33 of 4, 15 of 8 for 148 SMs. Heads of 64 have two CTAs an SM.
 int tk_attn_kv8_prefill_clusters(int D, int P, int n, int sm_count) {
-    if (D == 64) return (2 * sm_count - (n > 2 ? 16 : 0)) / n;
+    if (D == 64) return k8_clusters(2, sm_count, n);
     int clusters = 0;
     if ((P == 8 ? kp_clusters<128, 8>(n, &clusters) : kp_clusters<128, 16>(n, &clusters)) != cudaSuccess) {
         cudaGetLastError();

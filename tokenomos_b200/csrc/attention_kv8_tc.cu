@@ -524,7 +524,7 @@ struct K8tLaunch {
 };
 
 // How many clusters of `n` CTAs the device holds at once, asked for once. Where an SM holds one CTA, clusters lie in whole parts of the device, 15 of 8 or 33 of 4, not 148
-// SMs' worth, and the occupancy calculator knows. (It answers one CTA an SM for every kernel that allocates tensor memory, so what several need is counted here.)
+// SMs' worth, and the occupancy calculator knows.
 struct K8tPlaces {
     int n;
     int* clusters;
@@ -538,7 +538,7 @@ struct K8tPlaces {
         if (device < 16 && (*clusters = known[device][n].load(std::memory_order_relaxed)) > 0) return e;
         if constexpr (K8tSmem<D, NR, KG>::PER_SM > 1) {
             e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-            *clusters = K8tSmem<D, NR, KG>::PER_SM * sms / n;
+            *clusters = k8_clusters(K8tSmem<D, NR, KG>::PER_SM, sms, n);
         } else {
             cudaLaunchConfig_t cfg;
             cudaLaunchAttribute attr[2];
@@ -566,7 +566,8 @@ cudaError_t k8t_pick(int G, int D, int P, const F& f) {
 // How many CTAs share each of `items` tokens' keys, when no sequence holds more than `longest` positions and a query sees at most `reach` of them: as many as keep
 // every CTA resident (one CTA more and the launch runs in two waves), in clusters of at most eight with two tiles of 128 keys each, or of 16 with four (us by
 // shares, 8 KV heads of 64: a token behind 2,048 positions 14.9 unshared, 8.7 by 4, 7.6 by 8, 8.5 by 16; behind 30,000 136, 40, 24.7, 20.8; 8 tokens behind 32,000 49.0
-// by 6, 45.7 by 8, 61.7 by 10; 16 behind 4,000 15.3 by 4, 20.3 by 5; 64 behind up to 3,000 33.1 unshared, 38.9 by 2. One KV head of 128 with 16 query heads, whose CTA fills
+// by 6, 45.7 by 8, 61.7 by 10; 16 behind 4,000 15.3 by 4, 20.3 by 5; 64 behind up to 3,000 33.1 unshared, 38.9 by 2; one KV head: 30 tokens behind 9,000 14.7 by 8, 20.9 by 16, 72 behind
+// 4,000 13.5 by 7, 18.4 by 8. One KV head of 128 with 16 query heads, whose CTA fills
 // an SM: 18 tokens behind 30,000 51.2 by 6, 76.8 by 8, 82.2 by 16; 64 behind 3,000 33.0 unshared, 24.7 by 2, 33.6 by 4).
 TK_API int tk_attn_kv8_tc_splits(int items, int H, int Hkv, int D, int P, int longest, int reach) {
     const int64_t ctas = (int64_t)items * Hkv, keys = longest < reach ? longest : reach, tiles = (keys + 127) / 128 + (reach < longest ? 1 : 0);

@@ -61,6 +61,14 @@ inline bool k8_map(CUtensorMap* map, const void* pool, int D, int box_rows) {
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// How many clusters of n CTAs are resident at once where an SM holds per_sm of them, two or more. Pairs fill the device; larger clusters leave places empty, by measurement (148 SMs; the time of a
+// launch jumps by half where one cluster more has to wait): with two CTAs an SM 92 clusters of 3 run together, 70 of 4, 56 of 5, 45 of 6, 37 of 7, 33 of 8, 14 of 16; with four 185, 140, 112, 92, 76, 66
+// and 28. (The occupancy calculator cannot be asked: it answers one CTA an SM for every kernel that allocates tensor memory, and is exact for those that have no more.)
+inline int k8_clusters(int per_sm, int sm_count, int n) {
+    constexpr int EMPTY[9] = {0, 0, 0, 10, 8, 10, 13, 18, 16};             // SMs' worth, by cluster size
+    return per_sm * (sm_count - (n <= 8 ? EMPTY[n] : 36)) / n;
+}
+
 // programmatic dependent launch and, for more than one share, a cluster of that many CTAs; returns how many attributes
 inline int k8_attributes(cudaLaunchAttribute* attr, int cluster) {
     int n = 0;
